@@ -23,6 +23,14 @@ from .functional import (  # noqa: F401
     LogicLayerCudaFunction,
     TreeLogicFunction,
 )
+from .losses import (  # noqa: F401
+    BalanceLoss,
+    DistillationLoss,
+    TopLogits,
+    balance_loss,
+    distillation_loss,
+    top_logits,
+)
 from .model import ConvLogicCifarModel, ConvLogicMnistModel  # noqa: F401
 from .compiled_model import CompiledLogicNet  # noqa: F401
 from ._lib import LIB_PATH, W_ARGMAX, W_PROB, W_SOFTMAX  # noqa: F401
@@ -31,5 +39,6 @@ __all__ = [
     "ConvLogicLayer", "PoolLogicLayer", "TreeLogicLayer", "LogicLayer", "GroupSum", "PackBitsTensor",
     "ConvLogicFunction", "FullConvLogicFunction", "TreeLogicFunction", "LogicLayerCudaFunction", "GradFactor",
     "ConvLogicCifarModel", "ConvLogicMnistModel", "get_unique_connections", "CompiledLogicNet", "FusedLogicLayers", "fuse_logic_layers",
-    "GroupSumCrossEntropy", "FlatAdam", "GradBucket",
+    "GroupSumCrossEntropy", "FlatAdam", "GradBucket", "TopLogits", "top_logits", "distillation_loss", "DistillationLoss", "balance_loss",
+    "BalanceLoss",
 ]

@@ -16,7 +16,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "csrc", "libconvlogic_b200.so")
 BIND_PATH = os.path.join(_HERE, "csrc", "_clb_torch.so")
 
-F32, F64 = 0, 1
+F32, F64, F16, BF16 = 0, 1, 2, 3
+REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+TOP_MAX, BALANCE_MAX_EXPERTS, BALANCE_MAX_TOP = 128, 1024, 32
 W_PROB, W_SOFTMAX, W_ARGMAX = 0, 1, 2
 SEL_UNBOUNDED = 0x100
 Y_FEATURE_MAJOR = 0x200   # wmode flag: the block's output / upstream gradient is [C][windows][N]
@@ -99,6 +101,13 @@ _SIGNATURES = {
     "clb_group_sum_scratch_bytes": ([_i64, _i64, _i, _i], _sz),
     "clb_group_sum_fwd": ([_vp, _vp, _vp, _sz, _i64, _i64, _i, C.c_double, _i, _vp], _i),
     "clb_group_sum_ce": ([_vp] * 6 + [_sz, _i64, _i64, _i, C.c_double, _vp], _i),
+    "clb_top_logits": ([_vp, _i64] + [_vp] * 3 + [_i64, _i64, _i, C.c_double, _i, _vp], _i),
+    "clb_distill_scratch_bytes": ([_i64, _i64, _i], _sz),
+    "clb_distill_fwd": ([_vp, _i64] + [_vp] * 8 + [_sz, _i64, _i64, _i, C.c_double, _i, _i, _vp], _i),
+    "clb_distill_bwd": ([_vp, _i64] + [_vp] * 4 + [_i, _vp, _i64, _i64, _i, C.c_double, _i, _vp], _i),
+    "clb_balance_scratch_bytes": ([_i64, _i64], _sz),
+    "clb_balance_fwd": ([_vp, _i64] + [_vp] * 5 + [_sz, _i64, _i64, _i, _i, _vp], _i),
+    "clb_balance_bwd": ([_vp, _i64] + [_vp] * 4 + [_i64, _i64, _i, _vp], _i),
     "clb_transpose_f32": ([_vp, _vp, _i64, _i64, _vp], _i),
     "clb_adam_step": ([_vp] * 4 + [_i64] + [C.c_double] * 5 + [_i64, _i, _vp], _i),
     "clb_group_sum_bwd_scaled": ([_vp, _vp, _vp, _i64, _i64, _i, C.c_double, _i, _vp], _i),

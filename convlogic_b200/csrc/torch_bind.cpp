@@ -13,6 +13,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -1001,6 +1002,307 @@ Tensor trees(const Tensor &x, const Tensor &w0, const Tensor &w1, const Tensor &
     return out;
 }
 
+// ------------------------------------------------------------------------------------------------ loss terms on rows of scores
+int score_dtype(const Tensor &x)
+{
+    switch (x.scalar_type()) {
+    case at::kFloat: return CLB_F32;
+    case at::kHalf: return CLB_F16;
+    case at::kBFloat16: return CLB_BF16;
+    default: TORCH_CHECK(false, "convlogic_b200: expected float32, float16 or bfloat16 scores, got ", x.scalar_type());
+    }
+}
+
+// x [..., classes] as rows: read where it lies if its values do so one after the other and its rows at one distance, else from a copy.
+struct Rows {
+    Tensor x; // [rows, classes]
+    int64_t rows, classes, stride;
+    int dtype;
+};
+Rows rows_of(const Tensor &x, const char *what)
+{
+    TORCH_CHECK(x.is_cuda(), "convlogic_b200: tensor must be a CUDA tensor");
+    TORCH_CHECK(x.layout() == at::kStrided && x.dim() >= 1, "convlogic_b200: ", what, " must be [..., classes]");
+    TORCH_CHECK_VALUE(x.size(-1) > 0, "convlogic_b200: ", what, " have no classes");
+    const int64_t classes = x.size(-1), rows = x.numel() / classes;
+    Rows out{Tensor(), rows, classes, classes, score_dtype(x)};
+    // (a row of one class, or a tensor of one row, may have any stride there)
+    out.x = classes == 1 || x.stride(-1) == 1 ? x.reshape({rows, classes}) : x.contiguous().view({rows, classes});
+    if (classes > 1 && out.x.stride(1) != 1) out.x = out.x.contiguous();
+    out.stride = rows > 1 ? out.x.stride(0) : classes;
+    return out;
+}
+std::vector<int64_t> row_shape(const Tensor &x) { return {x.sizes().begin(), x.sizes().end() - 1}; }
+std::vector<int64_t> row_shape(const Tensor &x, int64_t last)
+{
+    std::vector<int64_t> s = row_shape(x);
+    s.push_back(last);
+    return s;
+}
+void check_temperature(double t) { TORCH_CHECK_VALUE(t >= 1e-30 && t <= 1e30, "convlogic_b200: the temperature must be positive and finite (1e-30 to 1e30), got ", t); }
+void check_top(int64_t k, int64_t classes)
+{
+    TORCH_CHECK_VALUE(k >= 1 && k <= classes, "convlogic_b200: the list must have 1 to ", classes, " of the ", classes, " classes, got ", k);
+    TORCH_CHECK_VALUE(k <= CLB_TOP_MAX, "convlogic_b200: lists have at most ", CLB_TOP_MAX, " classes, got ", k);
+}
+
+std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor &x_in, int64_t k, double temperature)
+{
+    check_temperature(temperature);
+    at::NoGradGuard no_grad;
+    const Rows x = rows_of(x_in, "the logits");
+    check_top(k, x.classes);
+    Below below(x.x);
+    Tensor values = alloc(row_shape(x_in, k), x.x, at::kFloat), indices = alloc(row_shape(x_in, k), x.x, at::kLong), rest = alloc(row_shape(x_in), x.x, at::kFloat);
+    if (x.rows)
+        check(clb_top_logits(ptr(x.x), x.stride, ptr<float>(values), ptr<int64_t>(indices), ptr<float>(rest), x.rows, x.classes, (int)k, temperature, x.dtype,
+                             cur_stream()));
+    return {values, indices, rest};
+}
+
+// A teacher's lists as the kernels read them.
+struct Lists {
+    Tensor values, indices, rest, weight;
+    int64_t k;
+};
+Lists lists_of(const Tensor &scores, const Tensor &values, const Tensor &indices, const std::optional<Tensor> &rest, const std::optional<Tensor> &weight)
+{
+    TORCH_CHECK_VALUE(values.dim() == scores.dim() && indices.dim() == scores.dim(), "convlogic_b200: the lists must be [..., k] for scores of ", scores.sizes());
+    const int64_t k = values.size(-1);
+    TORCH_CHECK_VALUE(k >= 1, "convlogic_b200: the lists are empty");
+    TORCH_CHECK_VALUE(k <= CLB_TOP_MAX, "convlogic_b200: lists have at most ", CLB_TOP_MAX, " classes, got ", k);
+    const std::vector<int64_t> want = row_shape(scores, k), per_row = row_shape(scores);
+    TORCH_CHECK_VALUE(values.sizes() == at::IntArrayRef(want) && indices.sizes() == at::IntArrayRef(want), "convlogic_b200: the lists must be ",
+                      at::IntArrayRef(want), ", got values ", values.sizes(), " and indices ", indices.sizes());
+    TORCH_CHECK(at::isFloatingType(values.scalar_type()), "convlogic_b200: the lists' values must be floating-point, got ", values.scalar_type());
+    TORCH_CHECK(indices.scalar_type() == at::kLong, "convlogic_b200: the lists' indices must be int64, got ", indices.scalar_type());
+    Lists out{Tensor(), Tensor(), Tensor(), Tensor(), k};
+    auto prepared = [&](const Tensor &t, const char *what, at::ScalarType type) {
+        TORCH_CHECK(t.device() == scores.device(), "convlogic_b200: ", what, " must be on ", scores.device(), ", got ", t.device());
+        TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), "convlogic_b200: ", what, " gets no gradient: detach it");
+        return t.detach().to(type).contiguous();
+    };
+    out.values = prepared(values, "the lists' values", at::kFloat);
+    out.indices = prepared(indices, "the lists' indices", at::kLong);
+    for (const auto &[t, what, to] : {std::tuple{&rest, "the rest's mass", &out.rest}, std::tuple{&weight, "the weight", &out.weight}}) {
+        if (!t->has_value()) continue;
+        TORCH_CHECK_VALUE((*t)->sizes() == at::IntArrayRef(per_row), "convlogic_b200: ", what, " must be ", at::IntArrayRef(per_row), ", got ", (*t)->sizes());
+        TORCH_CHECK(at::isFloatingType((*t)->scalar_type()), "convlogic_b200: ", what, " must be floating-point, got ", (*t)->scalar_type());
+        *to = prepared(**t, what, at::kFloat);
+    }
+    return out;
+}
+
+struct Distilled {
+    Tensor loss, stats, listed;
+};
+Distilled distill_fwd(const Rows &x, const Tensor &like, const Lists &l, double temperature, int reduction)
+{
+    Below below(x.x);
+    Distilled out;
+    out.loss = reduction == CLB_REDUCE_NONE ? alloc(row_shape(like), x.x, at::kFloat) : alloc({}, x.x, at::kFloat);
+    out.stats = alloc({x.rows, 2}, x.x, at::kFloat), out.listed = alloc({x.rows, l.k}, x.x, at::kFloat);
+    if (x.rows == 0 && reduction == CLB_REDUCE_NONE) return out;
+    const size_t bytes = clb_distill_scratch_bytes(x.rows, x.classes, (int)l.k);
+    Tensor scratch = scratch_bytes(bytes, x.x);
+    check(clb_distill_fwd(ptr(x.x), x.stride, ptr<float>(l.values), ptr<int64_t>(l.indices), ptr<float>(l.rest), ptr<float>(l.weight), ptr<float>(out.loss),
+                          ptr<float>(out.stats), ptr<float>(out.listed), ptr(scratch), bytes, x.rows, x.classes, (int)l.k, temperature, reduction, x.dtype,
+                          cur_stream()));
+    return out;
+}
+Tensor distill_bwd(const Rows &x, at::IntArrayRef sizes, const Tensor &indices, const Tensor &stats, const Tensor &listed, const Tensor &up, bool per_row,
+                   double temperature)
+{
+    Below below(x.x);
+    Tensor g = alloc(sizes, x.x);
+    if (x.rows)
+        check(clb_distill_bwd(ptr(x.x), x.stride, ptr<int64_t>(indices), ptr<float>(stats), ptr<float>(listed), ptr<float>(up), per_row, ptr(g), x.rows,
+                              x.classes, (int)listed.size(1), temperature, x.dtype, cur_stream()));
+    return g;
+}
+
+// The gradient of a node that can be differentiated once: under create_graph it hangs on a node that raises when a second derivative comes to it on
+// its way to `x`.
+variable_list once(Tensor g, const Tensor &x)
+{
+    if (at::GradMode::is_enabled() && x.requires_grad()) {
+        auto node = std::make_shared<torch::autograd::Error>("convlogic_b200: this loss can be differentiated once", torch::autograd::collect_next_edges(x));
+        torch::autograd::set_history(g, node);
+    }
+    return {g};
+}
+
+struct DistillNode : public Node {
+    SavedVariable x, indices, stats, listed;
+    int reduction;
+    double temperature;
+    std::string name() const override { return "DistillationFunctionBackward"; }
+    void release_variables() override { x.reset_data(), indices.reset_data(), stats.reset_data(), listed.reset_data(); }
+    variable_list apply(variable_list &&grads) override
+    {
+        const Tensor xx = x.unpack();
+        c10::cuda::CUDAGuard device(xx.device());
+        const Tensor up = upstream(*this, grads).detach().to(at::kFloat).contiguous();
+        Tensor g;
+        {
+            at::NoGradGuard no_grad;
+            g = distill_bwd(rows_of(xx, "the scores"), xx.sizes(), indices.unpack(), stats.unpack(), listed.unpack(), up, reduction == CLB_REDUCE_NONE,
+                            temperature);
+        }
+        return once(g, xx);
+    }
+};
+
+int reduction_code(const std::string &name)
+{
+    if (name == "none") return CLB_REDUCE_NONE;
+    if (name == "mean") return CLB_REDUCE_MEAN;
+    TORCH_CHECK_VALUE(name == "sum", "convlogic_b200: the reduction must be \"none\", \"mean\" or \"sum\", got \"", name, "\"");
+    return CLB_REDUCE_SUM;
+}
+
+Tensor distillation_loss(const Tensor &x_in, const Tensor &values, const Tensor &indices, const std::optional<Tensor> &rest,
+                         const std::optional<Tensor> &weight, double temperature, const std::string &reduction)
+{
+    if (followed({x_in})) return in_python("followed_distillation_loss", x_in, values, indices, rest, weight, temperature, reduction).cast<Tensor>();
+    const int how = reduction_code(reduction);
+    check_temperature(temperature);
+    Distilled out;
+    Lists l;
+    {
+        const Tensor plain = x_in.detach();
+        const Rows x = rows_of(plain, "the scores");
+        l = lists_of(x_in, values, indices, rest, weight);
+        out = distill_fwd(x, plain, l, temperature, how);
+    }
+    if (wants_grad({x_in})) {
+        auto node = new_node<DistillNode>();
+        node->set_next_edges(torch::autograd::collect_next_edges(x_in));
+        node->x = saved(x_in), node->indices = saved(l.indices), node->stats = saved(out.stats), node->listed = saved(out.listed);
+        node->reduction = how, node->temperature = temperature;
+        torch::autograd::set_history(out.loss, node);
+    }
+    return out.loss;
+}
+
+// the same for callers that handle autograd themselves: (loss, stats, listed), and the gradient from them
+std::tuple<Tensor, Tensor, Tensor> distill_fwd_py(const Tensor &x_in, const Tensor &values, const Tensor &indices, const std::optional<Tensor> &rest,
+                                                  const std::optional<Tensor> &weight, double temperature, const std::string &reduction)
+{
+    at::NoGradGuard no_grad;
+    const int how = reduction_code(reduction);
+    check_temperature(temperature);
+    const Rows x = rows_of(x_in, "the scores");
+    Distilled out = distill_fwd(x, x_in, lists_of(x_in, values, indices, rest, weight), temperature, how);
+    return {out.loss, out.stats, out.listed};
+}
+Tensor distill_bwd_py(const Tensor &up, const Tensor &x_in, const Tensor &indices, const Tensor &stats, const Tensor &listed, double temperature)
+{
+    at::NoGradGuard no_grad;
+    check_temperature(temperature);
+    const Rows x = rows_of(x_in, "the scores");
+    need_inputs(up, indices, stats, listed);
+    TORCH_CHECK(listed.dim() == 2 && listed.size(0) == x.rows && listed.size(1) >= 1 && listed.size(1) <= CLB_TOP_MAX && stats.numel() == 2 * x.rows &&
+                    indices.numel() == listed.numel() && indices.scalar_type() == at::kLong && stats.scalar_type() == at::kFloat &&
+                    listed.scalar_type() == at::kFloat,
+                "convlogic_b200: distill_bwd expects what distill_fwd returned for these scores");
+    TORCH_CHECK(up.scalar_type() == at::kFloat && (up.dim() == 0 || up.numel() == x.rows),
+                "convlogic_b200: the upstream gradient must be one float32 value, or one for each row");
+    return distill_bwd(x, x_in.sizes(), indices, stats, listed, up, up.dim() != 0, temperature);
+}
+
+// ---- balance over experts
+struct Balanced {
+    Tensor loss, counts, share, keep;
+};
+Balanced balance_fwd(const Rows &x, const Tensor &like, int64_t k, const std::optional<Tensor> &keep)
+{
+    TORCH_CHECK_VALUE(x.classes <= CLB_BALANCE_MAX_EXPERTS, "convlogic_b200: at most ", CLB_BALANCE_MAX_EXPERTS, " experts, got ", x.classes);
+    TORCH_CHECK_VALUE(k >= 1 && k <= x.classes && k <= CLB_BALANCE_MAX_TOP, "convlogic_b200: a row chooses 1 to ",
+                      std::min<int64_t>(x.classes, CLB_BALANCE_MAX_TOP), " of ", x.classes, " experts, got ", k);
+    Balanced out;
+    if (keep) {
+        const std::vector<int64_t> want = row_shape(like);
+        TORCH_CHECK(keep->scalar_type() == at::kBool, "convlogic_b200: `keep` must be bool, got ", keep->scalar_type());
+        TORCH_CHECK(keep->device() == like.device(), "convlogic_b200: `keep` must be on ", like.device(), ", got ", keep->device());
+        TORCH_CHECK_VALUE(keep->sizes() == at::IntArrayRef(want), "convlogic_b200: `keep` must be ", at::IntArrayRef(want), ", got ", keep->sizes());
+        out.keep = keep->contiguous();
+    }
+    Below below(x.x);
+    out.loss = alloc({}, x.x, at::kFloat), out.counts = alloc({x.classes}, x.x, at::kLong), out.share = alloc({x.classes}, x.x, at::kFloat);
+    const size_t bytes = clb_balance_scratch_bytes(x.rows, x.classes);
+    Tensor scratch = scratch_bytes(bytes, x.x);
+    check(clb_balance_fwd(ptr(x.x), x.stride, ptr<uint8_t>(out.keep), ptr<float>(out.loss), ptr<int64_t>(out.counts), ptr<float>(out.share), ptr(scratch), bytes,
+                          x.rows, x.classes, (int)k, x.dtype, cur_stream()));
+    return out;
+}
+Tensor balance_bwd(const Rows &x, at::IntArrayRef sizes, const Tensor &keep, const Tensor &share, const Tensor &up)
+{
+    Below below(x.x);
+    Tensor g = alloc(sizes, x.x);
+    if (x.rows)
+        check(clb_balance_bwd(ptr(x.x), x.stride, ptr<uint8_t>(keep), ptr<float>(share), ptr<float>(up), ptr(g), x.rows, x.classes, x.dtype, cur_stream()));
+    return g;
+}
+
+struct BalanceNode : public Node {
+    SavedVariable x, keep, share;
+    bool has_keep;
+    std::string name() const override { return "BalanceFunctionBackward"; }
+    void release_variables() override { x.reset_data(), keep.reset_data(), share.reset_data(); }
+    variable_list apply(variable_list &&grads) override
+    {
+        const Tensor xx = x.unpack();
+        c10::cuda::CUDAGuard device(xx.device());
+        const Tensor up = upstream(*this, grads).detach().to(at::kFloat).contiguous();
+        Tensor g;
+        {
+            at::NoGradGuard no_grad;
+            g = balance_bwd(rows_of(xx, "the logits"), xx.sizes(), has_keep ? keep.unpack() : Tensor(), share.unpack(), up);
+        }
+        return once(g, xx);
+    }
+};
+
+std::tuple<Tensor, Tensor> balance_loss(const Tensor &x_in, int64_t k, const std::optional<Tensor> &keep)
+{
+    if (followed({x_in})) return in_python("followed_balance_loss", x_in, k, keep).cast<std::tuple<Tensor, Tensor>>();
+    if (g_sinks.load(std::memory_order_relaxed) > 0 && x_in.requires_grad()) {
+        py::gil_scoped_acquire gil;
+        TORCH_CHECK(!sink_of(x_in), "convlogic_b200: these logits' gradient is written straight into a bucket by their layer (GradBucket.direct), "
+                                    "which would overwrite the balance loss's: turn it off with direct(False)");
+    }
+    Balanced out;
+    {
+        const Tensor plain = x_in.detach();
+        out = balance_fwd(rows_of(plain, "the logits"), plain, k, keep);
+    }
+    if (wants_grad({x_in})) {
+        auto node = new_node<BalanceNode>();
+        node->set_next_edges(torch::autograd::collect_next_edges(x_in));
+        node->x = saved(x_in), node->share = saved(out.share), node->has_keep = out.keep.defined();
+        if (out.keep.defined()) node->keep = saved(out.keep);
+        torch::autograd::set_history(out.loss, node);
+    }
+    return {out.loss, out.counts};
+}
+std::tuple<Tensor, Tensor, Tensor> balance_fwd_py(const Tensor &x_in, int64_t k, const std::optional<Tensor> &keep)
+{
+    at::NoGradGuard no_grad;
+    Balanced out = balance_fwd(rows_of(x_in, "the logits"), x_in, k, keep);
+    return {out.loss, out.counts, out.share};
+}
+Tensor balance_bwd_py(const Tensor &up, const Tensor &x_in, const Tensor &share, const std::optional<Tensor> &keep)
+{
+    at::NoGradGuard no_grad;
+    const Rows x = rows_of(x_in, "the logits");
+    need_inputs(up, share);
+    TORCH_CHECK(share.numel() == x.classes && share.scalar_type() == at::kFloat && up.numel() == 1 && up.scalar_type() == at::kFloat &&
+                    x.classes <= CLB_BALANCE_MAX_EXPERTS && (!keep || (keep->is_cuda() && keep->is_contiguous() && keep->scalar_type() == at::kBool && keep->numel() == x.rows)),
+                "convlogic_b200: balance_bwd expects what balance_fwd took and returned for these logits");
+    return balance_bwd(x, x_in.sizes(), keep.value_or(Tensor()), share, up);
+}
+
 // ------------------------------------------------------------------------------------------------ optimiser
 void adam_step(const Tensor &p, const Tensor &g, const Tensor &m, const Tensor &v, double lr, double beta1, double beta2, double eps, double weight_decay,
                int64_t step, bool decoupled)
@@ -1207,6 +1509,13 @@ PYBIND11_MODULE(_clb_torch, m)
     m.def("group_sum", &group_sum);
     m.def("group_sum_ce", &group_sum_ce);
     m.def("trees", &trees);
+    m.def("top_logits", &top_logits);
+    m.def("distillation_loss", &distillation_loss);
+    m.def("distill_fwd", &distill_fwd_py);
+    m.def("distill_bwd", &distill_bwd_py);
+    m.def("balance_loss", &balance_loss);
+    m.def("balance_fwd", &balance_fwd_py);
+    m.def("balance_bwd", &balance_bwd_py);
     m.def("transpose2d", &transpose2d);
     m.def("adam_step", &adam_step);
     m.def("count_sinks", [](int64_t change) { g_sinks += change; });

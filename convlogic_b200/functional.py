@@ -275,6 +275,38 @@ class LogicTreeCrossEntropyFunction(Function):
         return (gx, g0, g1, g2) + (None,) * 8
 
 
+class DistillationFunction(Function):
+    """Loss of scores against a teacher's lists of top logits (``ops.distill_fwd``); the lists and the weight get no gradient."""
+
+    @staticmethod
+    def forward(ctx, scores, values, indices, rest, weight, temperature, reduction):
+        loss, stats, listed = ops.distill_fwd(scores, values, indices, rest, weight, temperature, reduction)
+        ctx.save_for_backward(scores, indices, stats, listed)
+        ctx.temperature = temperature
+        return loss
+
+    @staticmethod
+    def backward(ctx, gloss):
+        scores, indices, stats, listed = ctx.saved_tensors
+        return (ops.distill_bwd(gloss.float(), scores, indices, stats, listed, ctx.temperature),) + (None,) * 6
+
+
+class BalanceFunction(Function):
+    """(balance loss, counts) of rows of logits over experts (``ops.balance_fwd``); the gradient goes through the probabilities."""
+
+    @staticmethod
+    def forward(ctx, logits, top_k, keep):
+        loss, counts, share = ops.balance_fwd(logits, top_k, keep)
+        ctx.save_for_backward(logits, share, keep)
+        ctx.mark_non_differentiable(counts)
+        return loss, counts
+
+    @staticmethod
+    def backward(ctx, gloss, unused):
+        logits, share, keep = ctx.saved_tensors
+        return ops.balance_bwd(gloss.float(), logits, share, keep), None, None
+
+
 class FeatureMajorFunction(Function):
     """[batch, features] -> contiguous [features, batch] (and the same copy back for the gradient) with the library's
     tiled transpose instead of a strided torch copy: the layout change in front of the flat layers."""
@@ -320,3 +352,11 @@ def followed_trees(x, w0, w1, w2, leaf, node, start, slots, wmode, covers_all, l
     if labels is None:
         return LogicTreeFunction.apply(x_fm, w0, w1, w2, leaf, node, start, slots, wmode, covers_all).transpose(0, 1)
     return LogicTreeCrossEntropyFunction.apply(x_fm, w0, w1, w2, leaf, node, start, slots, labels, k, tau, covers_all)
+
+
+def followed_distillation_loss(*args):
+    return DistillationFunction.apply(*args)
+
+
+def followed_balance_loss(*args):
+    return BalanceFunction.apply(*args)

@@ -497,3 +497,29 @@ def transpose2d(x):
 def adam_step(p, g, m, v, lr, beta1, beta2, eps, weight_decay, step, decoupled):
     """One Adam / AdamW step over flat fp32 buffers, in place."""
     native().adam_step(p, g, m, v, float(lr), float(beta1), float(beta2), float(eps), float(weight_decay), int(step), bool(decoupled))
+
+
+# ------------------------------------------------------------------------------------------- loss terms on rows of scores
+def top_logits(x, k, temperature=1.0):
+    """(values [..., k], indices [..., k], rest [...]) of the k largest logits of every row (see ``convlogic_b200.top_logits``)."""
+    return native().top_logits(x, k, temperature)
+
+
+def distill_fwd(scores, values, indices, rest=None, weight=None, temperature=1.0, reduction="mean"):
+    """(loss, stats, listed) of ``convlogic_b200.distillation_loss``: the last two are what ``distill_bwd`` needs beside the scores."""
+    return native().distill_fwd(scores, values, indices, rest, weight, temperature, reduction)
+
+
+def distill_bwd(gloss, scores, indices, stats, listed, temperature=1.0):
+    """Gradient of ``distill_fwd`` w.r.t. the scores; ``gloss`` float32, a scalar, or one value for each row (reduction "none")."""
+    return native().distill_bwd(gloss.contiguous(), scores, indices.contiguous(), stats, listed, temperature)
+
+
+def balance_fwd(logits, top_k=1, keep=None):
+    """(loss, counts, share) of ``convlogic_b200.balance_loss``: ``share`` is what ``balance_bwd`` needs beside the logits."""
+    return native().balance_fwd(logits, top_k, keep)
+
+
+def balance_bwd(gloss, logits, share, keep=None):
+    """Gradient of ``balance_fwd``'s loss w.r.t. the logits."""
+    return native().balance_bwd(gloss.contiguous(), logits, share, None if keep is None else keep.contiguous())

@@ -44,6 +44,9 @@ extern "C" {
 
 #define CLB_F32 0
 #define CLB_F64 1
+/* half types, taken by the operators on rows of scores alone (clb_top_logits, clb_distill_*, clb_balance_*) */
+#define CLB_F16 2
+#define CLB_BF16 3
 
 #define CLB_W_PROB 0
 #define CLB_W_SOFTMAX 1
@@ -415,6 +418,51 @@ int clb_group_sum_bwd_scaled(const void *gout, const void *scale, void *gy, int6
  * scratch as for clb_group_sum_fwd.  k <= 32.  Feed dscore (times the upstream scalar) to clb_group_sum_bwd. */
 int clb_group_sum_ce(const float *y, const int64_t *labels, float *scores, float *dscore, float *loss, void *scratch,
                      size_t scratch_bytes, int64_t F, int64_t B, int k, double tau, void *stream);
+
+/* Loss terms on rows of scores (no counterpart in the reference).  dtype: CLB_F32, CLB_F16 or CLB_BF16, what x / scores hold and the gradients
+ * get; a row's values lie one after the other, row r begins at element r * row_stride (0 is allowed: the same row every time).  Gradients are
+ * dense, [rows][classes].  Sums, lists and losses are fp32.  Results are the same from call to call.
+ *
+ * clb_top_logits: per row the k largest of `classes` logits, values [rows][k] in descending order, indices int64 [rows][k]; equal
+ * values by index, NaN before every number.  rest [rows] = log of the sum of exp(x / temperature) over the classes that are not listed, -inf where
+ * there is none.  1 <= k <= min(classes, CLB_TOP_MAX), temperature from 1e-30 to 1e30. */
+#define CLB_TOP_MAX 128
+int clb_top_logits(const void *x, int64_t row_stride, float *values, int64_t *indices, float *rest, int64_t rows, int64_t classes, int k,
+                   double temperature, int dtype, void *stream);
+
+/* Loss of scores against a teacher's lists, temperature^2 KL(teacher || student) with all classes outside a row's list taken as one:
+ *   p, r = soft-max over (values / temperature, rest), q = softmax(scores / temperature), q_r = sum of q over the unlisted classes,
+ *   loss = temperature^2 weight [ sum_k p_k (log p_k - log q_{i_k}) + r (log r - log q_r) ]     (nothing for a probability of zero).
+ * rest [rows] may be NULL (the listed classes are then all that the teacher knows: r = 0), weight [rows] may be NULL (ones).  An entry of
+ * a list whose index is outside [0, classes) does not exist; an index that is listed twice has both entries' probability.  A row of weight zero, of no
+ * teacher mass or of scores that are all -inf adds nothing and gets a gradient of zero, whatever else it holds.
+ * reduction: CLB_REDUCE_NONE (loss [rows]), CLB_REDUCE_MEAN (loss [1], the sum divided by rows) or CLB_REDUCE_SUM (loss [1]); zero rows add up to zero.
+ * The forward leaves stats [rows][2] and listed [rows][k] for the backward.
+ * scratch: clb_distill_scratch_bytes; not needed for CLB_REDUCE_NONE.  1 <= k <= CLB_TOP_MAX.
+ * clb_distill_bwd: grad = upstream * d loss / d scores; upstream is one float, or one for each row (upstream_per_row). */
+#define CLB_REDUCE_NONE 0
+#define CLB_REDUCE_MEAN 1
+#define CLB_REDUCE_SUM 2
+size_t clb_distill_scratch_bytes(int64_t rows, int64_t classes, int k);
+int clb_distill_fwd(const void *scores, int64_t row_stride, const float *values, const int64_t *indices, const float *rest, const float *weight,
+                    float *loss, float *stats, float *listed, void *scratch, size_t scratch_bytes, int64_t rows, int64_t classes, int k,
+                    double temperature, int reduction, int dtype, void *stream);
+int clb_distill_bwd(const void *scores, int64_t row_stride, const int64_t *indices, const float *stats, const float *listed, const float *upstream,
+                    int upstream_per_row, void *grad, int64_t rows, int64_t classes, int k, double temperature, int dtype, void *stream);
+
+/* Balance loss over experts (the 16 operations of a layer's gates, the experts of a router): with p = softmax(x) and the k largest logits of a
+ * row its choices (equal ones by index, never a logit of -inf), counts[e] = rows that choose e, M = kept rows,
+ *   loss = experts / (M k) * sum_e counts[e] * mean of p_e over the kept rows.
+ * Kept are the rows with keep[r] != 0 (keep may be NULL: all) that have a logit above -inf; M = 0: loss 0.  counts int64 [experts], loss [1]; share
+ * [experts] is what the backward needs: grad = upstream * p_j (share_j - sum_e p_e share_e), the gradient through p, zero for rows that are not kept.
+ * experts <= CLB_BALANCE_MAX_EXPERTS, 1 <= k <= min(experts, CLB_BALANCE_MAX_TOP), rows < 2^31. */
+#define CLB_BALANCE_MAX_EXPERTS 1024
+#define CLB_BALANCE_MAX_TOP 32
+size_t clb_balance_scratch_bytes(int64_t rows, int64_t experts);
+int clb_balance_fwd(const void *x, int64_t row_stride, const uint8_t *keep, float *loss, int64_t *counts, float *share, void *scratch,
+                    size_t scratch_bytes, int64_t rows, int64_t experts, int k, int dtype, void *stream);
+int clb_balance_bwd(const void *x, int64_t row_stride, const uint8_t *keep, const float *share, const float *upstream, void *grad, int64_t rows,
+                    int64_t experts, int dtype, void *stream);
 
 /* out [cols][rows] = transpose of in [rows][cols], fp32, out != in.  The copy between the [batch][features] tensors of
  * the conv blocks / the caller and the feature-major [features][batch] activations of the flat layers (the reference
