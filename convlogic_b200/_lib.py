@@ -103,8 +103,8 @@ _SIGNATURES = {
     "clb_group_sum_ce": ([_vp] * 6 + [_sz, _i64, _i64, _i, C.c_double, _vp], _i),
     "clb_top_logits": ([_vp, _i64] + [_vp] * 3 + [_i64, _i64, _i, C.c_double, _i, _vp], _i),
     "clb_distill_scratch_bytes": ([_i64, _i64, _i], _sz),
-    "clb_distill_fwd": ([_vp, _i64] + [_vp] * 8 + [_sz, _i64, _i64, _i, C.c_double, _i, _i, _vp], _i),
-    "clb_distill_bwd": ([_vp, _i64] + [_vp] * 4 + [_i, _vp, _i64, _i64, _i, C.c_double, _i, _vp], _i),
+    "clb_distill_fwd": ([_vp, _i64] + [_vp] * 9 + [_sz, _i64, _i64, _i, C.c_double, _i, _i, _vp], _i),
+    "clb_distill_bwd": ([_vp, _i64] + [_vp] * 4 + [_i, _i, _vp, _i64, _i64, _i, C.c_double, _i, _vp], _i),
     "clb_balance_scratch_bytes": ([_i64, _i64], _sz),
     "clb_balance_fwd": ([_vp, _i64] + [_vp] * 5 + [_sz, _i64, _i64, _i, _i, _vp], _i),
     "clb_balance_bwd": ([_vp, _i64] + [_vp] * 4 + [_i64, _i64, _i, _vp], _i),

@@ -71,7 +71,7 @@ extern "C" int clb_top_logits(const void *x, int64_t row_stride, float *values, 
 {
     if (!x || !values || !indices || !rest || rows < 0 || classes <= 0 || row_stride < 0 || k <= 0 || !(temperature >= 1e-30 && temperature <= 1e30)) return CLB_ERR_ARG;
     if (k > classes) return CLB_ERR_SHAPE;
-    if (k > CLB_TOP_MAX || classes > 0x7fffffff) return CLB_ERR_TOO_LARGE;
+    if (k > CLB_TOP_MAX || classes > CLB_CLASSES_MAX) return CLB_ERR_TOO_LARGE;
     if (dtype != CLB_F32 && dtype != CLB_F16 && dtype != CLB_BF16) return CLB_ERR_ARG;
     if (rows == 0) return CLB_OK;
     cudaStream_t st = (cudaStream_t)stream;

@@ -1094,30 +1094,31 @@ Lists lists_of(const Tensor &scores, const Tensor &values, const Tensor &indices
 }
 
 struct Distilled {
-    Tensor loss, stats, listed;
+    Tensor loss, stats, listed, grad;
 };
-Distilled distill_fwd(const Rows &x, const Tensor &like, const Lists &l, double temperature, int reduction)
+Distilled distill_fwd(const Rows &x, const Tensor &like, const Lists &l, double temperature, int reduction, bool want_grad = false)
 {
     Below below(x.x);
     Distilled out;
     out.loss = reduction == CLB_REDUCE_NONE ? alloc(row_shape(like), x.x, at::kFloat) : alloc({}, x.x, at::kFloat);
     out.stats = alloc({x.rows, 2}, x.x, at::kFloat), out.listed = alloc({x.rows, l.k}, x.x, at::kFloat);
     if (x.rows == 0 && reduction == CLB_REDUCE_NONE) return out;
+    if (want_grad) out.grad = alloc(like.sizes(), x.x);
     const size_t bytes = clb_distill_scratch_bytes(x.rows, x.classes, (int)l.k);
     Tensor scratch = scratch_bytes(bytes, x.x);
     check(clb_distill_fwd(ptr(x.x), x.stride, ptr<float>(l.values), ptr<int64_t>(l.indices), ptr<float>(l.rest), ptr<float>(l.weight), ptr<float>(out.loss),
-                          ptr<float>(out.stats), ptr<float>(out.listed), ptr(scratch), bytes, x.rows, x.classes, (int)l.k, temperature, reduction, x.dtype,
+                          ptr<float>(out.stats), ptr<float>(out.listed), ptr(out.grad), ptr(scratch), bytes, x.rows, x.classes, (int)l.k, temperature, reduction, x.dtype,
                           cur_stream()));
     return out;
 }
 Tensor distill_bwd(const Rows &x, at::IntArrayRef sizes, const Tensor &indices, const Tensor &stats, const Tensor &listed, const Tensor &up, bool per_row,
-                   double temperature)
+                   double temperature, Tensor unit = Tensor())
 {
     Below below(x.x);
-    Tensor g = alloc(sizes, x.x);
+    Tensor g = unit.defined() ? unit : alloc(sizes, x.x);
     if (x.rows)
-        check(clb_distill_bwd(ptr(x.x), x.stride, ptr<int64_t>(indices), ptr<float>(stats), ptr<float>(listed), ptr<float>(up), per_row, ptr(g), x.rows,
-                              x.classes, (int)listed.size(1), temperature, x.dtype, cur_stream()));
+        check(clb_distill_bwd(ptr(x.x), x.stride, ptr<int64_t>(indices), ptr<float>(stats), ptr<float>(listed), ptr<float>(up), per_row, unit.defined(),
+                              ptr(g), x.rows, x.classes, (int)listed.size(1), temperature, x.dtype, cur_stream()));
     return g;
 }
 
@@ -1132,12 +1133,36 @@ variable_list once(Tensor g, const Tensor &x)
     return {g};
 }
 
+// Which capture the current stream records into, 0 for none.
+unsigned long long capture_id()
+{
+    cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+    unsigned long long id = 0;
+    TORCH_CHECK(cudaStreamGetCaptureInfo(c10::cuda::getCurrentCUDAStream(), &status, &id) == cudaSuccess, "convlogic_b200: the stream cannot be asked for its capture");
+    return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
+// The forward writes the gradient for an upstream gradient of one while it holds the scores; the first backward call hands that tensor out, and its kernel
+// has work only if the upstream gradient is another.  A second call (retain_graph) takes the gradient from the scores, as does one that is not in the same
+// capture as the forward (or, like it, in none): a graph of the backward alone has to write its result at every replay, and a graph of the forward
+// would write over a result handed out.  Not for fp16, whose losses are scaled, nor for losses of rows.
 struct DistillNode : public Node {
     SavedVariable x, indices, stats, listed;
+    Tensor unit; // of the first backward call
+    unsigned long long capture = 0;
     int reduction;
     double temperature;
     std::string name() const override { return "DistillationFunctionBackward"; }
-    void release_variables() override { x.reset_data(), indices.reset_data(), stats.reset_data(), listed.reset_data(); }
+    void release_variables() override
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        x.reset_data(), indices.reset_data(), stats.reset_data(), listed.reset_data(), unit.reset();
+    }
+    Tensor take_unit()
+    {
+        std::lock_guard<std::mutex> lock(mutex_);
+        return unit.defined() && capture == capture_id() ? std::move(unit) : Tensor();
+    }
     variable_list apply(variable_list &&grads) override
     {
         const Tensor xx = x.unpack();
@@ -1147,7 +1172,7 @@ struct DistillNode : public Node {
         {
             at::NoGradGuard no_grad;
             g = distill_bwd(rows_of(xx, "the scores"), xx.sizes(), indices.unpack(), stats.unpack(), listed.unpack(), up, reduction == CLB_REDUCE_NONE,
-                            temperature);
+                            temperature, take_unit());
         }
         return once(g, xx);
     }
@@ -1169,17 +1194,22 @@ Tensor distillation_loss(const Tensor &x_in, const Tensor &values, const Tensor 
     check_temperature(temperature);
     Distilled out;
     Lists l;
+    const bool grad = wants_grad({x_in});
     {
         const Tensor plain = x_in.detach();
         const Rows x = rows_of(plain, "the scores");
         l = lists_of(x_in, values, indices, rest, weight);
-        out = distill_fwd(x, plain, l, temperature, how);
+        out = distill_fwd(x, plain, l, temperature, how, grad && how != CLB_REDUCE_NONE && x.dtype != CLB_F16);
     }
-    if (wants_grad({x_in})) {
+    if (grad) {
         auto node = new_node<DistillNode>();
         node->set_next_edges(torch::autograd::collect_next_edges(x_in));
         node->x = saved(x_in), node->indices = saved(l.indices), node->stats = saved(out.stats), node->listed = saved(out.listed);
-        node->reduction = how, node->temperature = temperature;
+        node->unit = out.grad, node->reduction = how, node->temperature = temperature;
+        if (out.grad.defined()) {
+            c10::cuda::CUDAGuard device(x_in.device());
+            node->capture = capture_id();
+        }
         torch::autograd::set_history(out.loss, node);
     }
     return out.loss;

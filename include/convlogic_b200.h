@@ -421,12 +421,13 @@ int clb_group_sum_ce(const float *y, const int64_t *labels, float *scores, float
 
 /* Loss terms on rows of scores (no counterpart in the reference).  dtype: CLB_F32, CLB_F16 or CLB_BF16, what x / scores hold and the gradients
  * get; a row's values lie one after the other, row r begins at element r * row_stride (0 is allowed: the same row every time).  Gradients are
- * dense, [rows][classes].  Sums, lists and losses are fp32.  Results are the same from call to call.
+ * dense, [rows][classes]; at most CLB_CLASSES_MAX classes.  Sums, lists and losses are fp32.  Results are the same from call to call.
  *
  * clb_top_logits: per row the k largest of `classes` logits, values [rows][k] in descending order, indices int64 [rows][k]; equal
  * values by index, NaN before every number.  rest [rows] = log of the sum of exp(x / temperature) over the classes that are not listed, -inf where
  * there is none.  1 <= k <= min(classes, CLB_TOP_MAX), temperature from 1e-30 to 1e30. */
 #define CLB_TOP_MAX 128
+#define CLB_CLASSES_MAX (1 << 30)
 int clb_top_logits(const void *x, int64_t row_stride, float *values, int64_t *indices, float *rest, int64_t rows, int64_t classes, int k,
                    double temperature, int dtype, void *stream);
 
@@ -437,18 +438,20 @@ int clb_top_logits(const void *x, int64_t row_stride, float *values, int64_t *in
  * a list whose index is outside [0, classes) does not exist; an index that is listed twice has both entries' probability.  A row of weight zero, of no
  * teacher mass or of scores that are all -inf adds nothing and gets a gradient of zero, whatever else it holds.
  * reduction: CLB_REDUCE_NONE (loss [rows]), CLB_REDUCE_MEAN (loss [1], the sum divided by rows) or CLB_REDUCE_SUM (loss [1]); zero rows add up to zero.
- * The forward leaves stats [rows][2] and listed [rows][k] for the backward.
+ * The forward leaves stats [rows][2] and listed [rows][k] for the backward, and writes d loss / d scores for an upstream gradient of one into grad, from
+ * the scores that it holds for the loss, unless grad is NULL.
  * scratch: clb_distill_scratch_bytes; not needed for CLB_REDUCE_NONE.  1 <= k <= CLB_TOP_MAX.
- * clb_distill_bwd: grad = upstream * d loss / d scores; upstream is one float, or one for each row (upstream_per_row). */
+ * clb_distill_bwd: grad = upstream * d loss / d scores; upstream is one float, or one for each row (upstream_per_row).  unit_done: the forward has written
+ * grad and nothing has changed it; where *upstream is 1, it is left as it is (not with upstream_per_row). */
 #define CLB_REDUCE_NONE 0
 #define CLB_REDUCE_MEAN 1
 #define CLB_REDUCE_SUM 2
 size_t clb_distill_scratch_bytes(int64_t rows, int64_t classes, int k);
 int clb_distill_fwd(const void *scores, int64_t row_stride, const float *values, const int64_t *indices, const float *rest, const float *weight,
-                    float *loss, float *stats, float *listed, void *scratch, size_t scratch_bytes, int64_t rows, int64_t classes, int k,
-                    double temperature, int reduction, int dtype, void *stream);
+                    float *loss, float *stats, float *listed, void *grad, void *scratch, size_t scratch_bytes, int64_t rows, int64_t classes,
+                    int k, double temperature, int reduction, int dtype, void *stream);
 int clb_distill_bwd(const void *scores, int64_t row_stride, const int64_t *indices, const float *stats, const float *listed, const float *upstream,
-                    int upstream_per_row, void *grad, int64_t rows, int64_t classes, int k, double temperature, int dtype, void *stream);
+                    int upstream_per_row, int unit_done, void *grad, int64_t rows, int64_t classes, int k, double temperature, int dtype, void *stream);
 
 /* Balance loss over experts (the 16 operations of a layer's gates, the experts of a router): with p = softmax(x) and the k largest logits of a
  * row its choices (equal ones by index, never a logit of -inf), counts[e] = rows that choose e, M = kept rows,

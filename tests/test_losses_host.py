@@ -40,14 +40,16 @@ def test_bad_arguments_are_refused_before_any_launch(lib):
     assert top(rows=0) == 0
 
     def fwd(loss=p, stats=p, listed=p, scratch=p, size=1 << 20, rows=4, classes=10, k=3, t=1.0, how=1, dtype=0, scores=p):
-        return lib.clb_distill_fwd(scores, 10, p, p, None, None, loss, stats, listed, scratch, size, rows, classes, k, t, how, dtype, None)
+        return lib.clb_distill_fwd(scores, 10, p, p, None, None, loss, stats, listed, None, scratch, size, rows, classes, k, t, how, dtype, None)
 
     for kw, want in (({"loss": None}, -1), ({"scores": None}, -1), ({"stats": None}, -1), ({"listed": None}, -1), ({"how": 3}, -1), ({"t": 0.0}, -1), ({"dtype": 1}, -1),
                      ({"k": 0}, -1), ({"rows": -1}, -1), ({"k": 129}, -6), ({"scratch": None}, -4), ({"size": 0}, -4)):
         assert fwd(**kw) == want, kw
     assert fwd(rows=0, how=0) == 0 and lib.clb_distill_scratch_bytes(0, 10, 3) == 0
-    assert lib.clb_distill_bwd(p, 10, p, p, p, None, 0, p, 4, 10, 3, 1.0, 0, None) == -1
-    assert lib.clb_distill_bwd(p, 10, p, p, p, p, 0, p, 0, 10, 3, 1.0, 0, None) == 0
+    assert lib.clb_distill_bwd(p, 10, p, p, p, None, 0, 0, p, 4, 10, 3, 1.0, 0, None) == -1
+    assert lib.clb_distill_bwd(p, 10, p, p, p, p, 0, 0, p, 0, 10, 3, 1.0, 0, None) == 0
+
+    assert lib.clb_distill_bwd(p, 10, p, p, p, p, 1, 1, p, 4, 10, 3, 1.0, 0, None) == -1     # rows' own upstream gradients are nothing that a forward knows
 
     def bal(loss=p, scratch=p, size=1 << 20, rows=4, experts=10, k=3, dtype=0, x=p):
         return lib.clb_balance_fwd(x, 10, None, loss, p, p, scratch, size, rows, experts, k, dtype, None)
