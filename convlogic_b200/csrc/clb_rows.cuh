@@ -70,9 +70,9 @@ template <typename T> struct RowPieces {
     __device__ __forceinline__ bool whole(int j) const { return first(j) >= 0 && first(j) <= classes - kPiece<T>; }
     __device__ __forceinline__ int piece_of(int cls) const { return (cls + phase) / kPiece<T>; }
     __device__ __forceinline__ int place_of(int cls) const { return (cls + phase) % kPiece<T>; }
-    __device__ __forceinline__ uint4 load(int j) const
+    // piece j, one that lies across an end of the row value by value
+    __device__ __forceinline__ uint4 edge(int j) const
     {
-        if (whole(j)) return __ldcs(reinterpret_cast<const uint4 *>(row + first(j)));
         uint32_t w[4] = {low_word<T>(), low_word<T>(), low_word<T>(), low_word<T>()};
         if (j < pieces)
 #pragma unroll
@@ -86,6 +86,37 @@ template <typename T> struct RowPieces {
             }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
+    // pieces j, j + step, ...: the whole ones are asked for before anything waits.  LAST: not read again
+    template <int NV, bool LAST = true> __device__ __forceinline__ void load(uint4 (&q)[NV], int j, int step) const
+    {
+        const T *const from = row + first(j);
+        auto get = [&](int i) {
+            const uint4 *p = reinterpret_cast<const uint4 *>(from + (long long)i * step * kPiece<T>);
+            return LAST ? __ldcs(p) : __ldg(p);
+        };
+        if (inside<NV>(j, step)) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) q[i] = get(i);
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            q[i] = make_uint4(low_word<T>(), low_word<T>(), low_word<T>(), low_word<T>());
+            if (whole(j + i * step)) q[i] = get(i);
+        }
+        if (j == 0 && !whole(0)) q[0] = edge(0); // (a first piece is some thread's first)
+        const int last = pieces - 1, i = last - j;
+        if (last > 0 && i >= 0 && i < NV * step && (i & (step - 1)) == 0 && !whole(last)) { // (step: a power of two)
+            const uint4 e = edge(last);
+#pragma unroll
+            for (int n = 0; n < NV; ++n) {
+                const bool here = n * step == i;
+                q[n].x = here ? e.x : q[n].x, q[n].y = here ? e.y : q[n].y, q[n].z = here ? e.z : q[n].z, q[n].w = here ? e.w : q[n].w;
+            }
+        }
+    }
+    // are pieces j, j + step, ..., NV of them, all whole?
+    template <int NV> __device__ __forceinline__ bool inside(int j, int step) const { return first(j) >= 0 && first(j + (NV - 1) * step) <= classes - kPiece<T>; }
     // writes a piece's values to the row `out` of as many classes; `aligned`: out has this row's phase
     __device__ __forceinline__ void store(T *out, bool aligned, int j, const uint4 &v) const
     {
@@ -104,39 +135,69 @@ template <typename T> struct RowPieces {
         }
     }
 };
+
 // value e of a piece becomes -inf
-template <typename T> __device__ __forceinline__ void drop_value(uint32_t (&w)[4], int e)
+template <typename T> __device__ __forceinline__ void drop_value(uint4 &q, int e)
 {
+    uint32_t w[4] = {q.x, q.y, q.z, q.w};
     if (sizeof(T) == 4) w[e & 3] = low_bits<T>();
     else w[e >> 1] = (e & 1) ? (w[e >> 1] & 0xffffu) | low_bits<T>() << 16 : (w[e >> 1] & 0xffff0000u) | low_bits<T>();
+    q = make_uint4(w[0], w[1], w[2], w[3]);
+}
+// sum of the exponentials of a piece's values with respect to R / c, in two chains
+template <typename T> __device__ __forceinline__ void piece_exp_sum(float (&l)[2], const uint4 &p, float R, float c)
+{
+    const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        float f[Word<T>::n];
+        Word<T>::get(w[q], f);
+#pragma unroll
+        for (int z = 0; z < Word<T>::n; ++z) l[(q + z) & 1] += ex2(fmaf(f[z], c, -R));
+    }
+}
+template <typename T> __device__ __forceinline__ uint32_t piece_max(uint32_t top, const uint4 &q)
+{
+    return Word<T>::max(Word<T>::max(top, Word<T>::max(q.x, q.y)), Word<T>::max(q.z, q.w));
+}
+template <typename T> __device__ __forceinline__ float word_max(uint32_t w)
+{
+    float f[Word<T>::n];
+    Word<T>::get(w, f);
+    return fmaxf(f[0], f[Word<T>::n - 1]);
 }
 
-// ---- sums and maxima over a team of TH threads
-template <int TH, bool MAX, int N> __device__ __forceinline__ void lanes_reduce(float (&v)[N])
+// ---- (m, l) of exponents over lanes
+__device__ __forceinline__ float exp_of(float v, float m, float c) { return ex2((v - m) * c); } // of v with respect to a finite m
+// One fused multiply-add a value instead of a difference and a product: exp((v - m) / T) = exp2(v c - R) * fix with R = m c, rounded, and fix = 2^(R - m c),
+// which the rounding of R left out.  Not where m c is beyond the largest float: a maximum of the type's lowest value (every class masked with it).
+struct ExpRef {
+    float R, fix;
+    bool far;
+};
+__device__ __forceinline__ ExpRef exp_ref(float m, float c)
 {
-#pragma unroll
-    for (int o = (TH < 32 ? TH : 32) / 2; o > 0; o >>= 1)
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const float other = __shfl_xor_sync(0xffffffffu, v[i], o);
-            v[i] = MAX ? fmaxf(v[i], other) : v[i] + other;
-        }
+    ExpRef r;
+    r.R = m * c, r.far = !(fabsf(m) < 1e38f && fabsf(r.R) < 1e38f), r.fix = ex2(-fmaf(m, c, -r.R));
+    return r;
 }
-// `red`: N * 32 floats of the block, not in use by an earlier reduction that some thread may still read
-template <int TH, bool MAX, int N> __device__ __forceinline__ void team_reduce(float (&v)[N], float *red)
+template <int LANES> __device__ __forceinline__ float lanes_max(float v)
 {
-    lanes_reduce<TH, MAX, N>(v);
-    if (TH > 32) {
-        constexpr int W = TH > 32 ? TH / 32 : 1;
-        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-        if (lane == 0)
 #pragma unroll
-            for (int i = 0; i < N; ++i) red[i * 32 + warp] = v[i];
-        __syncthreads();
+    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+template <int LANES> __device__ __forceinline__ float lanes_sum(float v)
+{
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = red[i * 32 + lane % W];
-        lanes_reduce<W, MAX, N>(v);
-    }
+    for (int o = LANES / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+// the lanes' exponents as one: every lane of LANES neighbours gets it
+template <int LANES> __device__ __forceinline__ ExpSum lanes_merge(ExpSum s, float c)
+{
+    const float m = lanes_max<LANES>(s.m);
+    return {m, lanes_sum<LANES>(s.l * exp_of(s.m, finite_or_zero(m), c))};
 }
 
 } // namespace clb

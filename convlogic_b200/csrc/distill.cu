@@ -25,218 +25,462 @@ struct DistillArgs {
     long long stride, rows;
     int classes, k;
     float temperature, c, scale; // c = log2(e) / T; scale: T, over the rows for a mean
+    int chunks, ranks_log;       // forward: how often a cluster comes back for more of a row; its blocks
 };
 
-template <typename T> struct Entry { // one class of a list: cls < 0: does not exist
+struct Entry { // one class of a list: cls < 0: does not exist
     int cls;
     float t, s;
 };
-template <typename T>
-__device__ __forceinline__ Entry<T> list_entry(const T *row, const int64_t *idx, const float *val, int n, int classes)
+
+// What a row's sums come to: unlisted scores `rest`, distinct listed ones `list`, the teacher's listed values `teach`, the teacher's rest rs, the weight.
+struct RowNumbers {
+    float m, coef, factor;              // unlisted gradient = coef * exp((s - m) / T); the list's = factor * (q - p)
+    float um, ul, tm, tl, re, log_rest; // all scores; the teacher's mass, exp(rest - tm); log of the unlisted scores' sum over ul's
+    bool there;
+    __device__ __forceinline__ float log_p(float t, float tt) const { return (t / tt - tm) - logf(tl); }
+    __device__ __forceinline__ float log_q(float s, float tt) const { return (s - um) / tt - logf(ul); }
+    __device__ __forceinline__ float loss(float listed, float rs, float tt) const
+    {
+        const float r = re / tl;
+        if (r > 0.f || r != r) listed += r * (((rs - tm) - logf(tl)) - log_rest);
+        return there ? listed * factor * tt : 0.f;
+    }
+};
+__device__ __forceinline__ RowNumbers row_numbers(ExpSum rest, ExpSum list, ExpSum teach, float rs, float w, const DistillArgs &a)
 {
-    const long long j = idx[n];
-    Entry<T> e{-1, -INFINITY, -INFINITY};
-    if (j >= 0 && j < classes) e.cls = (int)j, e.t = val[n], e.s = to_f(row[j]);
-    return e;
+    RowNumbers n;
+    const bool no_rest = rest.m == -INFINITY && rest.l == 0.f, no_list = list.m == -INFINITY && list.l == 0.f;
+    n.m = finite_or_zero(rest.m), n.um = finite_or_zero(fmaxf(rest.m, list.m));
+    const float of_rest = no_rest ? 0.f : rest.l * exp_of(n.m, n.um, a.c);
+    n.ul = of_rest + (no_list ? 0.f : list.l * exp_of(finite_or_zero(list.m), n.um, a.c));
+    const float tz = teach.m == -INFINITY ? -INFINITY : teach.m / a.temperature;
+    n.tm = finite_or_zero(fmaxf(tz, rs));
+    n.re = ex2((rs - n.tm) * 1.44269504f);
+    n.tl = (teach.m == -INFINITY ? teach.l : teach.l * ex2((tz - n.tm) * 1.44269504f)) + n.re;
+    n.there = w != 0.f && n.tl != 0.f && !(no_rest && no_list);
+    n.factor = w * a.scale;
+    n.coef = n.there && !no_rest ? n.factor * (__fdividef(of_rest, n.ul) - __fdividef(n.re, n.tl)) / rest.l : 0.f;
+    n.log_rest = no_rest ? -INFINITY : (n.m - n.um) / a.temperature + logf(rest.l) - logf(n.ul);
+    return n;
 }
+
+constexpr int kValues = 64; // of a row in a thread's registers, as fp32
 
 // TH threads a row (4 to 32: teams of a block of 256; more: the block), NV pieces a thread.  CLUSTER: the blocks of a cluster share a row.
 // grad: where d loss / d scores goes for an upstream gradient of one, or NULL.
+//
+// A thread takes the exponentials of its values with respect to its own maximum and keeps them, so that there is one exchange in the team, of pairs (maximum,
+// sum), and the gradient is the kept exponential times a factor of the thread's: one exponential a value.
 template <typename T, int TH, int NV, bool CLUSTER>
-__global__ void __launch_bounds__(TH <= 32 ? 256 : TH, TH <= 32 ? 4 : 1024 / TH)
+__global__ void __launch_bounds__(TH <= 32 ? 256 : TH, TH <= 32 ? 2 : 512 / TH)
     distill_fwd_kernel(const T *__restrict__ x, const float *__restrict__ values, const int64_t *__restrict__ indices, const float *__restrict__ rest,
                        const float *__restrict__ weight, float *__restrict__ row_loss, float *__restrict__ stats, float *__restrict__ listed, T *grad, DistillArgs a)
 {
     namespace cg = cooperative_groups;
-    constexpr int BLOCK = TH <= 32 ? 256 : TH, TEAMS = BLOCK / TH, EV = kPiece<T>, WORDS = NV * EV <= 32 ? 1 : 2; // bits of a thread's values
+    constexpr int BLOCK = TH <= 32 ? 256 : TH, TEAMS = BLOCK / TH, EV = kPiece<T>, LANES = TH < 32 ? TH : 32, WARPS = TH / LANES, RANKS = CLUSTER ? 8 : 1, WORDS = NV * EV <= 32 ? 1 : 2;
+    static_assert(NV * EV <= kValues, "a bit for each value");
     __shared__ uint32_t bits[WORDS][BLOCK];
-    __shared__ float red[3][3 * 32];
-    __shared__ float peer[2][16];
-    const int t = threadIdx.x % TH, team = threadIdx.x / TH;
-    const int ranks = CLUSTER ? (int)cg::this_cluster().num_blocks() : 1, rank = CLUSTER ? (int)cg::this_cluster().block_rank() : 0;
-    const long long groups = (long long)(gridDim.x / ranks) * TEAMS;
+    __shared__ int4 classes[TEAMS][CLB_TOP_MAX / 4]; // of the list, -1 behind its end
+    __shared__ ExpSum part[2][RANKS * WARPS]; // of the unlisted scores, for even and odd turns: each warp of each block of the cluster
+    __shared__ float4 list_part[4];           // of the list: maximum and sum of its scores, of the teacher's values
+    __shared__ float loss_part[4];
+    const int t = threadIdx.x % TH, team = threadIdx.x / TH, lane = threadIdx.x & 31, warp = t / 32;
+    const int ranks = CLUSTER ? 1 << a.ranks_log : 1, rank = CLUSTER ? blockIdx.x & (ranks - 1) : 0;
+    const int list_warps = TH > 32 ? (a.k + 31) / 32 : 1;
+    const int groups = (int)(gridDim.x >> (CLUSTER ? a.ranks_log : 0)) * TEAMS;
     auto team_sync = [] {
         if (TH <= 32) __syncwarp();
         else __syncthreads();
     };
-    if (CLUSTER) cg::this_cluster().barrier_arrive(); // no block writes to another's memory before that one runs
-    // every team of a warp takes every turn, on its last row again where it has none left
-    const long long turns = (a.rows + groups - 1) / groups;
-    for (long long turn = 0; turn < turns; ++turn) {
-        const long long r0 = turn * groups + (long long)(blockIdx.x / ranks) * TEAMS + team;
-        const bool live = r0 < a.rows;
-        const long long r = live ? r0 : a.rows - 1;
+    if (CLUSTER) { // no block writes to another's memory before that one runs and has cleared what a cluster of fewer blocks does not write
+        for (int i = threadIdx.x; i < 2 * RANKS * WARPS; i += BLOCK) part[0][i] = ExpSum{-INFINITY, 0.f};
+        cg::this_cluster().sync();
+    }
+    // (the teams of a warp take every turn together, on the last row again where one has none left)
+    const long long first_row = (long long)(blockIdx.x >> (CLUSTER ? a.ranks_log : 0)) * TEAMS;
+    const int of_warp = TH < 32 ? team & ~(32 / TH - 1) : team;
+    int turn = 0;
+    for (long long r_warp = first_row + of_warp; r_warp < a.rows; r_warp += groups, ++turn) {
+        const bool live = TH >= 32 || r_warp + (team - of_warp) < a.rows;
+        const long long r = live ? r_warp + (team - of_warp) : a.rows - 1;
         const RowPieces<T> row(x + r * a.stride, a.classes);
         const int64_t *idx = indices + r * a.k;
         const float *val = values + r * a.k;
+        const int chunks = CLUSTER ? a.chunks : 1; // (one unless the row is longer than the cluster's registers)
+        auto class_of = [&](int n) {
+            const long long j = idx[n];
+            return j >= 0 && j < a.classes ? (int)j : -1;
+        };
+        // (what lies elsewhere is asked for before the row)
         const float w = weight ? weight[r] : 1.f, rs = rest ? rest[r] : -INFINITY, tt = a.temperature;
-        const int chunks = TH <= 32 ? 1 : (row.pieces + ranks * TH * NV - 1) / (ranks * TH * NV);
-        uint32_t raw[NV][4];
-        bool twice = false;
-        Entry<T> own{-1, -INFINITY, -INFINITY};
-        if (t < a.k) own = list_entry(row.row, idx, val, t, a.classes);
-        auto entry = [&](int n) { return n == t ? own : list_entry(row.row, idx, val, n, a.classes); };
-        auto fetch = [&](int chunk) { // the thread's pieces, without the listed classes
+        Entry own{-1, -INFINITY, -INFINITY};
+        if (t < a.k) own.cls = class_of(t), own.t = val[t];
+        int *const list = reinterpret_cast<int *>(classes[team]);
+        auto entry = [&](int n) { // of the threads that hold the list, t + TH * i
+            if (n == t) return own;
+            Entry e{list[n], -INFINITY, -INFINITY};
+            if (e.cls >= 0) e.t = val[n], e.s = to_f(row.row[e.cls]);
+            return e;
+        };
+        float v[NV * EV]; // the thread's values, later their exponentials
+        auto fetch = [&](int chunk) {
             const int base = (chunk * ranks + rank) * TH * NV;
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const uint4 q = row.load(base + v * TH + t);
-                raw[v][0] = q.x, raw[v][1] = q.y, raw[v][2] = q.z, raw[v][3] = q.w;
-            }
+            uint4 raw[NV];
+            row.load(raw, base + t, TH);
 #pragma unroll
             for (int i = 0; i < WORDS; ++i) bits[i][threadIdx.x] = 0;
             team_sync();
-            for (int n = t; n < a.k; n += TH) {
-                const int cls = entry(n).cls;
+            for (int n = t; n < ((a.k + 3) & ~3); n += TH) { // the listed classes are struck out where they lie
+                const int cls = n == t ? own.cls : n < a.k ? class_of(n) : -1;
+                if (chunk == 0) list[n] = cls;
                 const int j = cls < 0 ? -1 : row.piece_of(cls) - base;
                 if (j < 0 || j >= TH * NV) continue;
                 const int bit = j / TH * EV + row.place_of(cls);
-                const uint32_t old = atomicOr(&bits[bit >> 5][team * TH + j % TH], 1u << (bit & 31));
-                twice = twice || ((old >> (bit & 31)) & 1);
+                atomicOr(&bits[bit >> 5][team * TH + j % TH], 1u << (bit & 31));
             }
+            if (chunk == 0 && own.cls >= 0) own.s = to_f(row.row[own.cls]);
             team_sync();
 #pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                const uint32_t m = bits[(v * EV) >> 5][threadIdx.x] >> ((v * EV) & 31);
-                if (m & ((1u << EV) - 1))
+            for (int i = 0; i < NV; ++i) {
+                const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-                    for (int e = 0; e < EV; ++e)
-                        if ((m >> e) & 1) drop_value<T>(raw[v], e);
+                for (int q = 0; q < 4; ++q) {
+                    float f[Word<T>::n];
+                    Word<T>::get(w[q], f);
+#pragma unroll
+                    for (int z = 0; z < Word<T>::n; ++z) v[i * EV + q * Word<T>::n + z] = f[z];
+                }
             }
+#pragma unroll
+            for (int half = 0; half < WORDS; ++half)
+                if (const uint32_t m = bits[half][threadIdx.x])
+#pragma unroll
+                    for (int i = half * 32; i < (half + 1) * 32 && i < NV * EV; ++i)
+                        if ((m >> (i & 31)) & 1) v[i] = -INFINITY;
         };
-        // ---- maxima: unlisted scores, listed scores, the teacher's list, and whether a class is listed twice
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, 0.f};
-        uint32_t top = low_word<T>();
+        auto exponentials = [&](float m) { // v = exp of v with respect to m; their sum
+            float l = 0.f;
+#pragma unroll
+            for (int i = 0; i < NV * EV; ++i) {
+                v[i] = exp_of(v[i], m, a.c);
+                l += v[i];
+            }
+            return l;
+        };
+        ExpSum mine{-INFINITY, 0.f};
         for (int ch = 0; ch < chunks; ++ch) {
             fetch(ch);
+            float m = v[0];
 #pragma unroll
-            for (int v = 0; v < NV; ++v)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top = Word<T>::max(top, raw[v][i]);
+            for (int i = 1; i < NV * EV; ++i) m = fmaxf(m, v[i]);
+            m = fmaxf(m, -INFINITY); // (NaN alone)
+            const float l = exponentials(finite_or_zero(m));
+            if (chunks == 1) mine = {m, l};
+            else mine = merge(mine, ExpSum{m, l}, a.c);
         }
-        {
-            float f[Word<T>::n];
-            Word<T>::get(top, f);
-#pragma unroll
-            for (int i = 0; i < Word<T>::n; ++i) mx[0] = fmaxf(mx[0], f[i]);
-        }
-        for (int n = t; n < a.k; n += TH) {
-            const Entry<T> e = entry(n);
-            mx[1] = fmaxf(mx[1], e.s), mx[2] = fmaxf(mx[2], e.t);
-        }
-        mx[3] = twice ? 1.f : 0.f;
-        team_reduce<TH, true, 4>(mx, red[0]);
-        if (CLUSTER) {
-            auto cl = cg::this_cluster();
-            if (turn == 0) cl.barrier_wait();
-            if (threadIdx.x < ranks) {
-                float *to = cl.map_shared_rank(&peer[0][0], threadIdx.x);
-                to[rank] = mx[0], to[8 + rank] = mx[3];
+        if (own.cls < 0) own.t = -INFINITY;
+        // ---- the list: distinct classes' scores, the teacher's values
+        float4 sums = make_float4(-INFINITY, 0.f, -INFINITY, 0.f);
+        uint32_t firsts = 0, twins = 0; // bit i: entry t + TH * i is the first of its class; its class is listed twice
+        auto compare = [&](int n, int cls) {
+            int before = 0, same = 0;
+            for (int o = 0; o < a.k; o += 4) {
+                const int4 q = classes[team][o / 4];
+                const int hits = (q.x == cls) + (q.y == cls) + (q.z == cls) + (q.w == cls);
+                same += hits;
+                before += o + 4 <= n ? hits : (q.x == cls && o < n) + (q.y == cls && o + 1 < n) + (q.z == cls && o + 2 < n);
             }
-            cl.sync();
-            for (int i = 0; i < ranks; ++i) mx[0] = fmaxf(mx[0], peer[0][i]), mx[3] = fmaxf(mx[3], peer[0][8 + i]);
-        }
-        const float m = finite_or_zero(mx[0]), mk = finite_or_zero(mx[1]), mt = finite_or_zero(mx[2]);
-        const bool dup = mx[3] != 0.f;
-        // ---- sums
-        float sum[3] = {0.f, 0.f, 0.f};
-        for (int ch = 0; ch < chunks; ++ch) {
-            if (chunks > 1) fetch(ch);
-            const int base = (ch * ranks + rank) * TH * NV;
-#pragma unroll
-            for (int v = 0; v < NV; ++v) {
-                if (base + v * TH >= row.pieces) break;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float f[Word<T>::n];
-                    Word<T>::get(raw[v][i], f);
-#pragma unroll
-                    for (int q = 0; q < Word<T>::n; ++q) sum[0] += ex2((f[q] - m) * a.c);
-                }
+            firsts |= (uint32_t)(before == 0) << (n / TH), twins |= (uint32_t)(same > 1) << (n / TH);
+        };
+        if (TH <= 32 || warp < list_warps) {
+            for (int n = t; n < a.k; n += TH) {
+                const Entry e = entry(n);
+                sums.x = fmaxf(sums.x, e.s), sums.z = fmaxf(sums.z, e.t);
             }
+            sums.x = lanes_max<LANES>(sums.x), sums.z = lanes_max<LANES>(sums.z);
+            for (int n = t; n < a.k; n += TH) {
+                const Entry e = entry(n);
+                if (e.cls < 0) continue;
+                compare(n, e.cls);
+                if ((firsts >> (n / TH)) & 1) sums.y += exp_of(e.s, finite_or_zero(sums.x), a.c);
+                sums.w += exp_of(e.t, finite_or_zero(sums.z), a.c);
+            }
+            sums.y = lanes_sum<LANES>(sums.y), sums.w = lanes_sum<LANES>(sums.w);
         }
-        for (int n = t; n < a.k; n += TH) {
-            const Entry<T> e = entry(n);
-            if (e.cls < 0) continue;
-            bool first = true;
-            if (dup)
-                for (int o = 0; o < n; ++o) first = first && idx[o] != e.cls;
-            if (first) sum[1] += expf((e.s - mk) / tt);
-            sum[2] += expf((e.t - mt) / tt);
+        // ---- the team's
+        const float own_max = mine.m;
+        mine = lanes_merge<LANES>(mine, a.c);
+        if (TH > 32) {
+            if (warp < list_warps && lane == 0) list_part[warp] = sums;
+            ExpSum *parts = part[turn & 1];
+            if (CLUSTER) {
+                if (lane < ranks) cg::this_cluster().map_shared_rank(parts, lane)[rank * WARPS + warp] = mine;
+                cg::this_cluster().sync();
+            } else {
+                if (lane == 0) parts[warp] = mine;
+                __syncthreads();
+            }
+            constexpr int N = RANKS * WARPS;
+            mine = parts[lane % N];
+#pragma unroll
+            for (int i = 32; i < N; i += 32) mine = merge(mine, parts[lane + i], a.c);
+            mine = lanes_merge<(N < 32 ? N : 32)>(mine, a.c);
+            ExpSum s{list_part[0].x, list_part[0].y}, u{list_part[0].z, list_part[0].w};
+            for (int i = 1; i < list_warps; ++i) {
+                s = merge(s, ExpSum{list_part[i].x, list_part[i].y}, a.c);
+                u = merge(u, ExpSum{list_part[i].z, list_part[i].w}, a.c);
+            }
+            sums = make_float4(s.m, s.l, u.m, u.l);
         }
-        team_reduce<TH, false, 3>(sum, red[1]);
-        if (CLUSTER) {
-            auto cl = cg::this_cluster();
-            if (threadIdx.x < ranks) cl.map_shared_rank(&peer[1][0], threadIdx.x)[rank] = sum[0];
-            cl.sync();
-            sum[0] = 0.f;
-            for (int i = 0; i < ranks; ++i) sum[0] += peer[1][i];
-        }
-        // ---- the row's numbers, in every thread
-        const bool no_rest = mx[0] == -INFINITY && sum[0] == 0.f, no_list = mx[1] == -INFINITY && sum[1] == 0.f;
-        const float um = finite_or_zero(fmaxf(mx[0], mx[1]));
-        const float ul = (no_rest ? 0.f : sum[0] * expf((m - um) / tt)) + (no_list ? 0.f : sum[1] * expf((mk - um) / tt));
-        const float tz = mx[2] == -INFINITY ? -INFINITY : mt / tt, tm = finite_or_zero(fmaxf(tz, rs));
-        const float tl = (mx[2] == -INFINITY ? sum[2] : sum[2] * expf(tz - tm)) + expf(rs - tm);
-        const bool there = w != 0.f && tl != 0.f && !(no_rest && no_list);
-        const float log_ul = logf(ul), log_tl = logf(tl);
-        const float lr = (rs - tm) - log_tl, rp = expf(lr);
-        const float lqr = no_rest ? -INFINITY : ((m - um) / tt + logf(sum[0])) - log_ul;
-        const float coef = there && !no_rest ? w * a.scale * (expf(lqr) - rp) / sum[0] : 0.f;
+        const RowNumbers num = row_numbers(mine, ExpSum{sums.x, sums.y}, ExpSum{sums.z, sums.w}, rs, w, a);
+        const float m = num.m, coef = num.coef;
         T *out = grad ? grad + r * a.classes : nullptr;
-        const bool aligned = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(row.row)) & 15) == 0;
-        if (grad)
+        if (grad) {
+            const bool aligned = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(row.row)) & 15) == 0;
             for (int ch = 0; ch < chunks; ++ch) {
-                if (chunks > 1) fetch(ch);
+                float scale = coef;
+                if (chunks == 1) scale = coef * exp_of(own_max, m, a.c);
+                else {
+                    fetch(ch);
+                    exponentials(m);
+                }
+                if (coef == 0.f) // (a row that adds nothing may hold NaN)
+#pragma unroll
+                    for (int i = 0; i < NV * EV; ++i) v[i] = 0.f;
                 const int base = (ch * ranks + rank) * TH * NV;
 #pragma unroll
-                for (int v = 0; v < NV; ++v) {
-                    const int j = base + v * TH + t;
-                    if (j >= row.pieces || !live) continue;
-                    uint4 q = make_uint4(0, 0, 0, 0);
-                    uint32_t *o = &q.x;
-                    if (coef != 0.f)
+                for (int i = 0; i < NV; ++i) {
+                    const int j = base + i * TH + t;
+                    uint32_t o[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            float f[Word<T>::n];
-                            Word<T>::get(raw[v][i], f);
+                    for (int q = 0; q < 4; ++q) {
+                        float f[Word<T>::n];
 #pragma unroll
-                            for (int z = 0; z < Word<T>::n; ++z) f[z] = coef * ex2((f[z] - m) * a.c);
-                            o[i] = Word<T>::put(f);
-                        }
-                    row.store(out, aligned, j, q);
+                        for (int z = 0; z < Word<T>::n; ++z) f[z] = scale * v[i * EV + q * Word<T>::n + z];
+                        o[q] = Word<T>::put(f);
+                    }
+                    if (j < row.pieces && live) row.store(out, aligned, j, make_uint4(o[0], o[1], o[2], o[3]));
                 }
-                }
-        // ---- the list: loss, and the gradient of its classes
-        if (grad) team_sync(); // a listed class is written after the piece that it lies in
-        float loss[1] = {0.f};
-        for (int n = t; n < a.k; n += TH) {
-            const Entry<T> e = entry(n);
-            float g = 0.f;
-            if (there && e.cls >= 0) {
-                const float lp = ((e.t / tt) - tm) - log_tl, lq = (e.s - um) / tt - log_ul, p = expf(lp);
-                if (p > 0.f || p != p) loss[0] += p * (lp - lq);
-                float mass = p;
-                if (dup) { // both entries' probability, in the list's order
-                    mass = 0.f;
-                    for (int o = 0; o < a.k; ++o)
-                        if (idx[o] == e.cls) mass += expf(((val[o] / tt) - tm) - log_tl);
-                }
-                g = w * a.scale * (expf(lq) - mass);
-            }
-            if (rank == 0 && live) listed[r * a.k + n] = g;
-            if (grad && live && e.cls >= 0) {
-                const int j = row.piece_of(e.cls) / (TH * NV);
-                if (!CLUSTER || j % ranks == rank) out[e.cls] = from_f<T>(g);
             }
         }
-        team_reduce<TH, false, 1>(loss, red[2]);
+        // ---- the list again: its loss, and the gradient of its classes
+        float loss = 0.f, own_grad = 0.f;
+        auto gradient_of = [&](int n, const Entry &e) {
+            if (!num.there || e.cls < 0) return 0.f;
+            const float lp = num.log_p(e.t, tt), lq = num.log_q(e.s, tt), p = expf(lp);
+            if (p > 0.f || p != p) loss += p * (lp - lq);
+            float mass = p;
+            if ((twins >> (n / TH)) & 1) { // a class that is listed twice has both entries' probability
+                mass = 0.f;
+                for (int o = 0; o < a.k; ++o)
+                    if (list[o] == e.cls) mass += expf(num.log_p(val[o], tt));
+            }
+            return num.factor * (expf(lq) - mass);
+        };
+        if (TH > 32) {
+            if (warp < list_warps) {
+                if (t < a.k) own_grad = gradient_of(t, own);
+                loss = lanes_sum<32>(loss);
+                if (lane == 0) loss_part[warp] = loss;
+            }
+            __syncthreads(); // a listed class is written after the piece that it lies in
+        } else
+            __syncwarp();
+        for (int n = t; n < a.k; n += TH) {
+            const Entry e = entry(n);
+            const float g = TH > 32 ? own_grad : gradient_of(n, e);
+            if (rank == 0 && live) listed[r * a.k + n] = g;
+            if (grad && live && e.cls >= 0 && (!CLUSTER || ((row.piece_of(e.cls) / (TH * NV)) & (ranks - 1)) == rank)) out[e.cls] = from_f<T>(g);
+        }
+        if (TH <= 32) loss = lanes_sum<LANES>(loss);
         if (t == 0 && rank == 0 && live) {
-            if (there && (rp > 0.f || rp != rp)) loss[0] += rp * (lr - lqr);
-            row_loss[r] = there ? loss[0] * w * a.scale * tt : 0.f;
+            if (TH > 32) {
+                loss = 0.f;
+                for (int i = 0; i < list_warps; ++i) loss += loss_part[i];
+            }
+            row_loss[r] = num.loss(loss, rs, tt);
             stats[2 * r] = m, stats[2 * r + 1] = coef;
         }
-        // (the tables are used again: each has a barrier of its team, or of the cluster, between the last read of this turn and the next turn's write)
+        team_sync(); // the tables are used again
+    }
+}
+
+// Rows that are longer than a block's registers, many of them: a block reads its row twice, the second time for the gradient and from the L2, backwards.  What
+// is in flight (two rows an SM, or one of more than 256 KB) has to fit there.
+// The bit of a listed class is in a table of the whole row; a thread's 64 or 32 values of a trip have a word of it.
+template <typename T, int TH>
+__global__ void __launch_bounds__(TH, 1024 / TH)
+    distill_stream_kernel(const T *__restrict__ x, const float *__restrict__ values, const int64_t *__restrict__ indices, const float *__restrict__ rest,
+                          const float *__restrict__ weight, float *__restrict__ row_loss, float *__restrict__ stats, float *__restrict__ listed, T *grad,
+                          DistillArgs a)
+{
+    constexpr int NV = 8, EV = kPiece<T>, WARPS = TH / 32, WORDS = NV * EV / 32;
+    extern __shared__ uint32_t struck[]; // [trips][WORDS][TH]
+    __shared__ int list[CLB_TOP_MAX];
+    __shared__ ExpSum part[WARPS];
+    __shared__ float4 list_part[4];
+    __shared__ float loss_part[4];
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, list_warps = (a.k + 31) / 32;
+    const float tt = a.temperature;
+    for (int i = t; i < a.chunks * WORDS * TH; i += TH) struck[i] = 0;
+    // a row's list and numbers are asked for while the row before it is written
+    long long next_cls = -1;
+    float next_t = -INFINITY, next_w = 1.f, next_rest = -INFINITY;
+    auto ask = [&](long long r) {
+        if (r >= a.rows) return;
+        if (t < a.k) next_cls = indices[r * a.k + t], next_t = values[r * a.k + t];
+        if (weight) next_w = weight[r];
+        if (rest) next_rest = rest[r];
+    };
+    ask(blockIdx.x);
+    __syncthreads();
+    for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const RowPieces<T> row(x + r * a.stride, a.classes);
+        const float w = next_w, rs = next_rest;
+        Entry own{-1, -INFINITY, -INFINITY};
+        int word = 0;
+        bool twice = false;
+        if (t < a.k && next_cls >= 0 && next_cls < a.classes) {
+            own.cls = (int)next_cls, own.t = next_t, own.s = to_f(row.row[own.cls]);
+            const int j = row.piece_of(own.cls), bit = j / TH % NV * EV + row.place_of(own.cls);
+            word = (j / (TH * NV) * WORDS + (bit >> 5)) * TH + j % TH;
+            twice = (atomicOr(&struck[word], 1u << (bit & 31)) >> (bit & 31)) & 1;
+        }
+        if (t < a.k) list[t] = own.cls;
+        const bool dup = __syncthreads_or(twice);
+        uint4 raw[NV];
+        auto strike = [&](int trip) {
+#pragma unroll
+            for (int h = 0; h < WORDS; ++h)
+                if (const uint32_t m = struck[(trip * WORDS + h) * TH + t])
+#pragma unroll
+                    for (int i = 0; i < NV / WORDS; ++i)
+#pragma unroll
+                        for (int e = 0; e < EV; ++e)
+                            if ((m >> (i * EV + e)) & 1) drop_value<T>(raw[h * (NV / WORDS) + i], e);
+        };
+        ExpSum mine{-INFINITY, 0.f};
+        for (int trip = 0; trip < a.chunks; ++trip) {
+            row.template load<NV, false>(raw, trip * TH * NV + t, TH);
+            strike(trip);
+            uint32_t top = low_word<T>();
+#pragma unroll
+            for (int i = 0; i < NV; ++i) top = piece_max<T>(top, raw[i]);
+            const float m = fmaxf(mine.m, word_max<T>(top)), ref = finite_or_zero(m);
+            const float before = mine.l * exp_of(mine.m, ref, a.c);
+            const ExpRef er = exp_ref(ref, a.c);
+            float l[2] = {0.f, 0.f};
+            if (!er.far) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) piece_exp_sum<T>(l, raw[i], er.R, a.c);
+                l[0] = (l[0] + l[1]) * er.fix;
+            } else {
+#pragma unroll 1
+                for (int i = 0; i < NV; ++i) {
+                    const uint4 p = raw[0];
+#pragma unroll
+                    for (int n = 1; n < NV; ++n) raw[n - 1] = raw[n];
+                    raw[NV - 1] = p; // (a rotation: no register is named by a number that varies)
+                    const uint32_t o[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        float f[Word<T>::n];
+                        Word<T>::get(o[q], f);
+#pragma unroll
+                        for (int z = 0; z < Word<T>::n; ++z) l[0] += exp_of(f[z], ref, a.c);
+                    }
+                }
+            }
+            mine = {m, before + l[0]};
+        }
+        // ---- the list and the row
+        bool first = own.cls >= 0;
+        if (dup && first)
+            for (int o = 0; o < t; ++o) first = first && list[o] != own.cls;
+        mine = lanes_merge<32>(mine, a.c);
+        if (lane == 0) part[warp] = mine;
+        if (warp < list_warps) {
+            float4 sums;
+            sums.x = lanes_max<32>(own.s), sums.z = lanes_max<32>(own.t);
+            sums.y = lanes_sum<32>(first ? exp_of(own.s, finite_or_zero(sums.x), a.c) : 0.f);
+            sums.w = lanes_sum<32>(own.cls >= 0 ? exp_of(own.t, finite_or_zero(sums.z), a.c) : 0.f);
+            if (lane == 0) list_part[warp] = sums;
+        }
+        __syncthreads();
+        mine = lanes_merge<WARPS>(part[lane % WARPS], a.c);
+        ExpSum sk{list_part[0].x, list_part[0].y}, tk{list_part[0].z, list_part[0].w};
+        for (int i = 1; i < list_warps; ++i) {
+            sk = merge(sk, ExpSum{list_part[i].x, list_part[i].y}, a.c);
+            tk = merge(tk, ExpSum{list_part[i].z, list_part[i].w}, a.c);
+        }
+        const RowNumbers n = row_numbers(mine, sk, tk, rs, w, a);
+        float own_grad = 0.f;
+        if (warp < list_warps) {
+            float loss = 0.f;
+            if (n.there && own.cls >= 0) {
+                const float lp = n.log_p(own.t, tt), lq = n.log_q(own.s, tt), p = expf(lp);
+                if (p > 0.f || p != p) loss = p * (lp - lq);
+                float mass = p;
+                if (dup) { // a class that is listed twice has both entries' probability
+                    mass = 0.f;
+                    for (int o = 0; o < a.k; ++o)
+                        if (list[o] == own.cls) mass += expf(n.log_p(values[r * a.k + o], tt));
+                }
+                own_grad = n.factor * (expf(lq) - mass);
+            }
+            loss = lanes_sum<32>(loss);
+            if (lane == 0) loss_part[warp] = loss;
+            if (t < a.k) listed[r * a.k + t] = own_grad;
+        }
+        next_cls = -1;
+        ask(r + gridDim.x);
+        T *out = grad ? grad + r * a.classes : nullptr;
+        if (grad) {
+            const bool aligned = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(row.row)) & 15) == 0;
+            const ExpRef er = exp_ref(n.m, a.c);
+            const float fixed = n.coef * er.fix;
+            for (int trip = a.chunks - 1; trip >= 0; --trip) {
+                const int base = trip * TH * NV + t;
+                if (trip < a.chunks - 1) {
+                    row.load(raw, base, TH);
+                    strike(trip);
+                }
+                auto gradients = [&](auto exponential) {
+                    const bool inside = aligned && row.template inside<NV>(base, TH);
+#pragma unroll
+                    for (int i = 0; i < NV; ++i) {
+                        uint32_t o[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) {
+                            float f[Word<T>::n];
+                            Word<T>::get(o[q], f);
+#pragma unroll
+                            for (int z = 0; z < Word<T>::n; ++z) f[z] = exponential(f[z]);
+                            o[q] = Word<T>::put(f);
+                        }
+                        const uint4 g = make_uint4(o[0], o[1], o[2], o[3]);
+                        if (inside) __stcs(reinterpret_cast<uint4 *>(out + row.first(base) + (long long)i * TH * EV), g);
+                        else if (base + i * TH < row.pieces) row.store(out, aligned, base + i * TH, g);
+                    }
+                };
+                if (n.coef == 0.f) gradients([](float) { return 0.f; }); // (a row that adds nothing may hold NaN)
+                else if (!er.far) gradients([&](float v) { return fixed * ex2(fmaf(v, a.c, -er.R)); });
+                else gradients([&](float v) { return n.coef * exp_of(v, n.m, a.c); });
+            }
+        }
+        __syncthreads(); // a listed class is written after the piece that it lies in
+        if (own.cls >= 0) {
+            if (grad) out[own.cls] = from_f<T>(own_grad);
+            struck[word] = 0;
+        }
+        if (t == 0) {
+            float loss = 0.f;
+            for (int i = 0; i < list_warps; ++i) loss += loss_part[i];
+            row_loss[r] = n.loss(loss, rs, tt);
+            stats[2 * r] = n.m, stats[2 * r + 1] = n.coef;
+        }
+        __syncthreads(); // the table is clear
     }
 }
 
@@ -259,8 +503,7 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const T *__restrict__ 
         T *out = gx + r * a.classes;
         const bool aligned = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(row.row)) & 15) == 0;
         uint4 raw[NV];
-#pragma unroll
-        for (int v = 0; v < NV; ++v) raw[v] = row.load(base + v * TH + t);
+        row.load(raw, base + t, TH);
         const float g = up[r * up_stride], m = stats[2 * r], coef = stats[2 * r + 1] * g;
 #pragma unroll
         for (int v = 0; v < NV; ++v) {
@@ -321,8 +564,10 @@ struct FwdPointers {
 };
 
 template <typename T, int TH, int NV, bool CLUSTER>
-cudaError_t launch_fwd(const T *x, const FwdPointers &p, T *grad, const DistillArgs &a, int cluster, cudaStream_t st)
+cudaError_t launch_fwd(const T *x, const FwdPointers &p, T *grad, DistillArgs a, int ranks_log, long long pieces, cudaStream_t st)
 {
+    const int cluster = 1 << ranks_log;
+    a.ranks_log = ranks_log, a.chunks = (int)((pieces + (long long)cluster * TH * NV - 1) / ((long long)cluster * TH * NV));
     constexpr int BLOCK = TH <= 32 ? 256 : TH, TEAMS = BLOCK / TH;
     const long long groups = (a.rows + TEAMS - 1) / TEAMS, most = (1 << 20) / cluster;
     cudaLaunchConfig_t cfg = {};
@@ -337,17 +582,37 @@ cudaError_t launch_fwd(const T *x, const FwdPointers &p, T *grad, const DistillA
                                        grad, a));
     return rc;
 }
+// pieces of the longest row: rows at a multiple of 16 bytes all begin at the first one's place in its piece
+template <typename T> long long most_pieces(const T *x, const DistillArgs &a)
+{
+    const int phase = a.rows == 1 || a.stride % kPiece<T> == 0 ? (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) : kPiece<T> - 1;
+    return ((long long)a.classes + phase + kPiece<T> - 1) / kPiece<T>;
+}
+template <typename T, int TH> cudaError_t launch_stream(const T *x, const FwdPointers &p, T *grad, DistillArgs a, long long pieces, cudaStream_t st)
+{
+    constexpr int NV = 8, WORDS = NV * kPiece<T> / 32;
+    a.chunks = (int)((pieces + TH * NV - 1) / (TH * NV));
+    const int bytes = a.chunks * WORDS * TH * 4;
+    const cudaError_t rc = ensure_dynamic_smem(distill_stream_kernel<T, TH>, bytes);
+    if (rc != cudaSuccess) return rc;
+    const long long most = (long long)sm_count() * (1024 / TH);
+    CLB_TRACED("distill_stream_kernel", st,
+               distill_stream_kernel<T, TH><<<(unsigned)(a.rows < most ? a.rows : most), TH, bytes, st>>>(x, p.values, p.indices, p.rest, p.weight, p.row_loss,
+                                                                                                        p.stats, p.listed, grad, a));
+    return cudaPeekAtLastError();
+}
 template <typename T> cudaError_t run_fwd(const T *x, const FwdPointers &p, T *grad, const DistillArgs &a, cudaStream_t st)
 {
-    const long long pieces = (a.classes + 2LL * kPiece<T> - 2) / kPiece<T>;
-    if (pieces <= 4) return launch_fwd<T, 4, 1, false>(x, p, grad, a, 1, st);
-    if (pieces <= 32) return launch_fwd<T, 8, 4, false>(x, p, grad, a, 1, st);
-    if (pieces <= 256) return launch_fwd<T, 32, 8, false>(x, p, grad, a, 1, st);
-    if (pieces <= 1024) return launch_fwd<T, 128, 8, false>(x, p, grad, a, 1, st);
-    if (pieces <= 2048) return launch_fwd<T, 256, 8, false>(x, p, grad, a, 1, st);
-    if (pieces <= 4096) return launch_fwd<T, 512, 8, false>(x, p, grad, a, 1, st);
-    if (pieces <= 8 * 4096) return launch_fwd<T, 512, 8, true>(x, p, grad, a, pieces <= 2 * 4096 ? 2 : pieces <= 4 * 4096 ? 4 : 8, st);
-    return launch_fwd<T, 1024, 8, true>(x, p, grad, a, 8, st);
+    constexpr int NV = kValues / kPiece<T>;
+    const long long pieces = most_pieces(x, a), block = 256 * NV;
+    if (pieces <= 4) return launch_fwd<T, 4, 1, false>(x, p, grad, a, 0, pieces, st);
+    if (pieces <= 8 * NV) return launch_fwd<T, 8, NV, false>(x, p, grad, a, 0, pieces, st);
+    if (pieces <= 32 * NV) return launch_fwd<T, 32, NV, false>(x, p, grad, a, 0, pieces, st);
+    if (pieces <= 128 * NV) return launch_fwd<T, 128, NV, false>(x, p, grad, a, 0, pieces, st);
+    if (pieces <= block) return launch_fwd<T, 256, NV, false>(x, p, grad, a, 0, pieces, st);
+    if (a.rows >= 64 && pieces <= 1200000 / kPiece<T>) return pieces <= 16384 ? launch_stream<T, 512>(x, p, grad, a, pieces, st) : launch_stream<T, 1024>(x, p, grad, a, pieces, st);
+    if (pieces <= 8 * block) return launch_fwd<T, 256, NV, true>(x, p, grad, a, pieces <= 2 * block ? 1 : pieces <= 4 * block ? 2 : 3, pieces, st);
+    return launch_fwd<T, 512, NV, true>(x, p, grad, a, 3, pieces, st);
 }
 
 template <typename T, int TH, int NV>
@@ -404,7 +669,7 @@ extern "C" int clb_distill_bwd(const void *scores, int64_t row_stride, const int
     with_score_type(dtype, [&](auto t) {
         using T = decltype(t);
         const DistillArgs a = make_args(rows, classes, row_stride, k, temperature, CLB_REDUCE_SUM);
-        const long long pieces = (classes + 2LL * kPiece<T> - 2) / kPiece<T>;
+        const long long pieces = most_pieces((const T *)scores, a);
         auto go = [&](auto launch) { launch((const T *)scores, indices, stats, listed, upstream, upstream_per_row ? 1 : 0, unit_done ? 1 : 0, (T *)grad, a, pieces, st); };
         if (pieces <= 4) go(launch_bwd<T, 4, 1>);
         else if (pieces <= 32) go(launch_bwd<T, 8, 4>);
