@@ -5,147 +5,283 @@
 //     loss = E / (M k) sum_e c_e P_e,  P_e = (1 / M) sum of p_e over the kept rows
 //     d loss / d x_j = p_j (h_j - sum_e p_e h_e),  h_e = E / (M^2 k) (c_e - mean of c)    (the counts have no gradient)
 // A constant taken off every h_e changes nothing; with the mean off, the difference of two nearly equal numbers in a balanced layer is taken in 64 bits.
-// Simple form: a warp per row.
-#include "clb_scores.cuh"
+//
+// G lanes (1 to 32) hold a row, 16 or 32 columns each and always the same ones, so that a lane adds up its columns' probabilities and counts in registers over
+// all its rows: no atomics, the same sums every time.  Both passes are bound by HBM (or by the L2 where the logits fit it); the backward pass goes
+// through the rows from the last one on, which is what the L2 still holds.
+#include <algorithm>
+#include <type_traits>
+
+#include "clb_rows.cuh"
 
 using namespace clb;
 using namespace clb_host;
 
 namespace {
 
-constexpr int kWarps = 8;
-constexpr int kMaxBlocks = 1024;
-constexpr int kSlots = CLB_BALANCE_MAX_EXPERTS / 32; // columns of a lane
+template <int NC> constexpr int kThreads = NC > 16 ? 128 : 256; // of a block (32 columns a lane: what four warps' sums take of shared memory)
+constexpr float kLog2e = 1.44269504f;
+constexpr uint32_t kMasked = 0x007fffffu; // order_key(-inf)
 
-int balance_blocks(long long rows) { return (int)(rows < (long long)kMaxBlocks * kWarps ? (rows + kWarps - 1) / kWarps : kMaxBlocks); }
-
-// the row's soft-max in place (columns lane, lane + 32, ...); false for a row that is not kept
-__device__ __forceinline__ bool row_softmax(float (&v)[kSlots], int lane, int experts)
+// The columns of lane t of G: pieces of 16 bytes (VEC: rows at multiples of 16 bytes, whole pieces), or every G-th column.  Ascending either way.
+template <typename T, int G, int NC, bool VEC> __device__ __forceinline__ int column(int i, int t)
 {
-    float m = -INFINITY;
-    bool nan = false;
-    for (int s = 0; s * 32 < experts; ++s) {
-        m = fmaxf(m, v[s]);
-        nan = nan || v[s] != v[s];
+    constexpr int EV = kPiece<T>;
+    return VEC ? (i / EV * G + t) * EV + i % EV : i * G + t;
+}
+template <typename T, int G, int NC, bool VEC> __device__ __forceinline__ void load_row(float (&v)[NC], const T *row, int t, int experts)
+{
+    constexpr int EV = kPiece<T>;
+    if constexpr (VEC) {
+        uint4 q[NC / EV];
+#pragma unroll
+        for (int i = 0; i < NC / EV; ++i) {
+            q[i] = make_uint4(low_word<T>(), low_word<T>(), low_word<T>(), low_word<T>());
+            if ((i * G + t) * EV < experts) q[i] = *reinterpret_cast<const uint4 *>(row + (i * G + t) * EV);
+        }
+#pragma unroll
+        for (int i = 0; i < NC / EV; ++i) {
+            const uint32_t w[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float f[Word<T>::n];
+                Word<T>::get(w[j], f);
+#pragma unroll
+                for (int z = 0; z < Word<T>::n; ++z) v[i * EV + j * Word<T>::n + z] = f[z];
+            }
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) v[i] = i * G + t < experts ? to_f(row[i * G + t]) : -INFINITY;
     }
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    if (m == -INFINITY && !__any_sync(0xffffffffu, nan)) return false;
+}
+// v becomes the row's probabilities; false for a row without a logit above -inf (NaN is one)
+template <int G, int NC> __device__ __forceinline__ bool soft_max(float (&v)[NC])
+{
+    float m = v[0];
+#pragma unroll
+    for (int i = 1; i < NC; ++i) m = fmaxf(m, v[i]);
+    m = lanes_max<G>(m);
+    const float ref = finite_or_zero(m);
     float l = 0.f;
-    for (int s = 0; s * 32 < experts; ++s) {
-        v[s] = lane + s * 32 < experts ? expf(v[s] - m) : 0.f;
-        l += v[s];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        v[i] = ex2((v[i] - ref) * kLog2e);
+        l += v[i];
     }
-    l = warp_sum<float>(l);
-    for (int s = 0; s * 32 < experts; ++s) v[s] /= l;
-    return true;
+    l = lanes_sum<G>(l);
+    const float inv = 1.f / l;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) v[i] *= inv;
+    return l != 0.f;
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kWarps * 32) balance_fwd_kernel(const T *__restrict__ x, long long stride, const uint8_t *__restrict__ keep,
-                                                                  float *__restrict__ sums, int *__restrict__ counts, int *__restrict__ kept, long long rows,
-                                                                  int experts, int k)
+template <typename T, int G, int NC, bool VEC>
+__global__ void __launch_bounds__(kThreads<NC>) balance_fwd_kernel(const T *__restrict__ x, long long stride, const uint8_t *__restrict__ keep,
+                                                               float *__restrict__ sums, int *__restrict__ counts, int *__restrict__ kept, int rows, int experts,
+                                                               int k)
 {
-    __shared__ float psum[CLB_BALANCE_MAX_EXPERTS];
-    __shared__ int cnt[CLB_BALANCE_MAX_EXPERTS], all;
-    for (int e = threadIdx.x; e < experts; e += kWarps * 32) psum[e] = 0.f, cnt[e] = 0;
-    if (threadIdx.x == 0) all = 0;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    float acc[kSlots];
-    int own[kSlots], mine = 0;
-    for (int s = 0; s < kSlots; ++s) acc[s] = 0.f, own[s] = 0;
-    for (long long r = (long long)blockIdx.x * kWarps + warp; r < rows; r += (long long)gridDim.x * kWarps) {
-        if (keep && !keep[r]) continue;
-        const T *row = x + r * stride;
-        float v[kSlots], raw[kSlots];
-        for (int s = 0; s * 32 < experts; ++s) raw[s] = v[s] = lane + s * 32 < experts ? to_f(row[lane + s * 32]) : -INFINITY;
-        if (!row_softmax(v, lane, experts)) continue;
-        ++mine;
-        for (int s = 0; s * 32 < experts; ++s) acc[s] += v[s];
-        unsigned long long last = ~0ull;
+    constexpr int TEAMS = kThreads<NC> / G, WARPS = kThreads<NC> / 32;
+    __shared__ float psum[WARPS][G * NC];
+    __shared__ int cnt[WARPS][G * NC], all[WARPS];
+    const int t = threadIdx.x % G, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    float acc[NC];
+    int own[NC], mine = 0;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) acc[i] = 0.f, own[i] = 0;
+    // the teams of a warp take their turns together
+    const int of_warp = blockIdx.x * TEAMS + (G < 32 ? warp * (32 / G) : warp);
+    for (long long r0 = of_warp; r0 < rows; r0 += (long long)gridDim.x * TEAMS) {
+        const long long r = r0 + lane / G;
+        const bool live = r < rows && (!keep || keep[r]);
+        float v[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) v[i] = -INFINITY;
+        if (live) load_row<T, G, NC, VEC>(v, x + r * stride, t, experts);
+        uint32_t key[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) key[i] = order_key(v[i]);
+        if (!soft_max<G, NC>(v)) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i) v[i] = 0.f, key[i] = 0;
+        } else
+            mine += t == 0;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) acc[i] += v[i];
         for (int n = 0; n < k; ++n) {
-            unsigned long long best = 0;
-            for (int s = 0; s * 32 < experts; ++s) {
-                const int e = lane + s * 32;
-                const unsigned long long p = ((unsigned long long)order_key(raw[s]) << 32) | (0xffffffffu - (uint32_t)e);
-                if (e < experts && raw[s] != -INFINITY && p < last && p > best) best = p;
+            uint32_t best = key[0];
+            int at = 0;
+#pragma unroll
+            for (int i = 1; i < NC; ++i)
+                if (key[i] > best) best = key[i], at = i;
+            uint32_t top = best;
+            int col = column<T, G, NC, VEC>(at, t);
+            if (G > 1) {
+#pragma unroll
+                for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                int first = best == top ? col : 0x7fffffff;
+#pragma unroll
+                for (int o = G / 2; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+                if (first != col || best != top) at = -1;
             }
-            for (int o = 16; o > 0; o >>= 1) {
-                const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
-                if (other > best) best = other;
-            }
-            if (!best) break;
-            last = best;
-            const uint32_t e = 0xffffffffu - (uint32_t)best;
-            if ((e & 31) == (uint32_t)lane) ++own[e >> 5];
+            if (top <= kMasked) at = -1; // nothing is left to choose
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                if (i == at) ++own[i], key[i] = 0;
         }
     }
-    for (int w = 0; w < kWarps; ++w) { // warps add in turn: the same sums every time
-        __syncthreads();
-        if (w == warp) {
-            for (int s = 0; s * 32 < experts; ++s)
-                if (lane + s * 32 < experts) psum[lane + s * 32] += acc[s], cnt[lane + s * 32] += own[s];
-            if (lane == 0) all += mine;
+    // the teams of a warp, then the warps, each in order
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+#pragma unroll
+        for (int o = 16; o >= G; o >>= 1) {
+            acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+            own[i] += __shfl_xor_sync(0xffffffffu, own[i], o);
         }
+        if (lane < G) psum[warp][column<T, G, NC, VEC>(i, t)] = acc[i], cnt[warp][column<T, G, NC, VEC>(i, t)] = own[i];
     }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    if (lane == 0) all[warp] = mine;
     __syncthreads();
-    for (int e = threadIdx.x; e < experts; e += kWarps * 32) {
-        sums[(long long)blockIdx.x * experts + e] = psum[e];
-        counts[(long long)blockIdx.x * experts + e] = cnt[e];
+    for (int e = threadIdx.x; e < experts; e += kThreads<NC>) {
+        float p = 0.f;
+        int c = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) p += psum[w][e], c += cnt[w][e];
+        sums[(long long)blockIdx.x * experts + e] = p;
+        counts[(long long)blockIdx.x * experts + e] = c;
     }
-    if (threadIdx.x == 0) kept[blockIdx.x] = all;
+    if (threadIdx.x == 0) {
+        int m = 0;
+        for (int w = 0; w < WARPS; ++w) m += all[w];
+        kept[blockIdx.x] = m;
+    }
 }
 
-__global__ void __launch_bounds__(256) balance_finish_kernel(const float *__restrict__ sums, const int *__restrict__ counts, const int *__restrict__ kept,
-                                                             float *__restrict__ loss, int64_t *__restrict__ total, float *__restrict__ share, int blocks,
-                                                             int experts, int k)
+// Adds up the blocks' sums: `per` threads an expert, each its share of the blocks in order.
+__global__ void __launch_bounds__(1024) balance_finish_kernel(const float *__restrict__ sums, const int *__restrict__ counts, const int *__restrict__ kept,
+                                                              float *__restrict__ loss, int64_t *__restrict__ total, float *__restrict__ share, int blocks,
+                                                              int experts, int per, int k)
 {
-    __shared__ double red[256];
-    double dot = 0.0, m = 0.0, picked = 0.0;
-    for (int b = 0; b < blocks; ++b) m += kept[b];
-    for (int e = threadIdx.x; e < experts; e += 256) {
-        double p = 0.0;
-        long long c = 0;
-        for (int b = 0; b < blocks; ++b) p += sums[(long long)b * experts + e], c += counts[(long long)b * experts + e];
-        total[e] = c;
-        dot += (double)c * p;
-        picked += (double)c;
-    }
-    for (int round = 0; round < 2; ++round) {
-        red[threadIdx.x] = round ? picked : dot;
-        __syncthreads();
-        for (int half = 128; half >= 1; half >>= 1) {
-            if ((int)threadIdx.x < half) red[threadIdx.x] += red[threadIdx.x + half];
-            __syncthreads();
-        }
-        if (round) picked = red[0];
-        else dot = red[0];
-        __syncthreads();
-    }
-    const double factor = m > 0.0 ? experts / (m * m * k) : 0.0;
-    if (threadIdx.x == 0) *loss = (float)(factor * dot);
-    for (int e = threadIdx.x; e < experts; e += 256) share[e] = (float)(factor * ((double)total[e] - picked / experts));
-}
-
-template <typename T>
-__global__ void __launch_bounds__(kWarps * 32) balance_bwd_kernel(const T *__restrict__ x, long long stride, const uint8_t *__restrict__ keep,
-                                                                  const float *__restrict__ share, const float *__restrict__ up, T *__restrict__ gx,
-                                                                  long long rows, int experts)
-{
+    __shared__ double ps[1024];
+    __shared__ long long cs[1024];
+    __shared__ double red[3][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    // thread = part * experts + e: neighbours read neighbouring experts
+    const int e = threadIdx.x % experts, part = threadIdx.x / experts;
+    double p = 0.0;
+    long long c = 0;
+    if (part < per)
+        for (int b = part; b < blocks; b += per) p += sums[(long long)b * experts + e], c += counts[(long long)b * experts + e];
+    ps[threadIdx.x] = p, cs[threadIdx.x] = c;
+    double m = 0.0;
+    for (int b = threadIdx.x; b < blocks; b += 1024) m += kept[b];
+    __syncthreads();
+    p = 0.0, c = 0;
+    if (threadIdx.x < experts)
+        for (int i = 0; i < per; ++i) p += ps[i * experts + threadIdx.x], c += cs[i * experts + threadIdx.x];
+    double v[3] = {(double)c * p, (double)c, m};
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    if (lane == 0)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) red[i][warp] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 3; ++i) v[i] = red[i][lane];
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int i = 0; i < 3; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], o);
+    const double factor = v[2] > 0.0 ? experts / (v[2] * v[2] * k) : 0.0;
+    if (threadIdx.x == 0) *loss = (float)(factor * v[0]);
+    if (threadIdx.x < experts) total[threadIdx.x] = c, share[threadIdx.x] = (float)(factor * ((double)c - v[1] / experts));
+}
+
+template <typename T, int G, int NC, bool VEC>
+__global__ void __launch_bounds__(kThreads<NC>) balance_bwd_kernel(const T *__restrict__ x, long long stride, const uint8_t *__restrict__ keep,
+                                                               const float *__restrict__ share, const float *__restrict__ up, T *__restrict__ gx, int rows,
+                                                               int experts)
+{
+    constexpr int TEAMS = kThreads<NC> / G, EV = kPiece<T>;
+    const int t = threadIdx.x % G, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const float g = *up;
-    for (long long r = (long long)blockIdx.x * kWarps + warp; r < rows; r += (long long)gridDim.x * kWarps) {
-        const T *row = x + r * stride;
-        float v[kSlots];
-        for (int s = 0; s * 32 < experts; ++s) v[s] = lane + s * 32 < experts ? to_f(row[lane + s * 32]) : -INFINITY;
-        const bool there = (!keep || keep[r]) && row_softmax(v, lane, experts);
-        float dot = 0.f;
-        if (there)
-            for (int s = 0; s * 32 < experts; ++s)
-                if (lane + s * 32 < experts) dot += v[s] * share[lane + s * 32];
-        dot = warp_sum<float>(dot);
-        for (int s = 0; s * 32 < experts; ++s)
-            if (lane + s * 32 < experts) gx[r * experts + lane + s * 32] = from_f<T>(there ? g * v[s] * (share[lane + s * 32] - dot) : 0.f);
+    float h[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int e = column<T, G, NC, VEC>(i, t);
+        h[i] = e < experts ? share[e] : 0.f;
     }
+    const int of_warp = blockIdx.x * TEAMS + (G < 32 ? warp * (32 / G) : warp);
+    for (long long r0 = of_warp; r0 < rows; r0 += (long long)gridDim.x * TEAMS) {
+        const long long r = rows - 1 - (r0 + lane / G);
+        const bool kept = r >= 0 && (!keep || keep[r]);
+        float v[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) v[i] = -INFINITY;
+        if (kept) load_row<T, G, NC, VEC>(v, x + r * stride, t, experts);
+        const bool there = soft_max<G, NC>(v) && kept;
+        float dot = 0.f;
+#pragma unroll
+        for (int i = 0; i < NC; ++i) dot += v[i] * h[i];
+        dot = lanes_sum<G>(dot);
+#pragma unroll
+        for (int i = 0; i < NC; ++i) v[i] = there ? g * (v[i] * (h[i] - dot)) : 0.f;
+        if (r < 0) continue;
+        T *out = gx + r * experts;
+        if constexpr (VEC) {
+#pragma unroll
+            for (int i = 0; i < NC / EV; ++i) {
+                uint32_t w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    float f[Word<T>::n];
+#pragma unroll
+                    for (int z = 0; z < Word<T>::n; ++z) f[z] = v[i * EV + j * Word<T>::n + z];
+                    w[j] = Word<T>::put(f);
+                }
+                if ((i * G + t) * EV < experts) __stcs(reinterpret_cast<uint4 *>(out + (i * G + t) * EV), make_uint4(w[0], w[1], w[2], w[3]));
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+                if (i * G + t < experts) out[i * G + t] = from_f<T>(v[i]);
+        }
+    }
+}
+
+// f(G, NC) for so many experts, as compile-time numbers: a thread a row up to 16, more lanes of 16 columns up to 512, then 32 columns
+template <typename F> void with_team(int64_t experts, F &&f)
+{
+    using std::integral_constant;
+    if (experts <= 4) f(integral_constant<int, 1>(), integral_constant<int, 8>());
+    else if (experts <= 8) f(integral_constant<int, 1>(), integral_constant<int, 8>());
+    else if (experts <= 16) f(integral_constant<int, 1>(), integral_constant<int, 16>());
+    else if (experts <= 32) f(integral_constant<int, 2>(), integral_constant<int, 16>());
+    else if (experts <= 64) f(integral_constant<int, 4>(), integral_constant<int, 16>());
+    else if (experts <= 128) f(integral_constant<int, 8>(), integral_constant<int, 16>());
+    else if (experts <= 256) f(integral_constant<int, 16>(), integral_constant<int, 16>());
+    else if (experts <= 512) f(integral_constant<int, 32>(), integral_constant<int, 16>());
+    else f(integral_constant<int, 32>(), integral_constant<int, 32>());
+}
+int teams_of(int64_t experts) // of a block
+{
+    int n = 0;
+    with_team(experts, [&](auto G, auto NC) { n = kThreads<decltype(NC)::value> / decltype(G)::value; });
+    return n;
+}
+// Blocks of the forward pass: up to six an SM, and sums of at most 512 KB for the one block that finishes.
+int balance_blocks(int64_t rows, int64_t experts)
+{
+    const int64_t teams = teams_of(experts), most = std::min<int64_t>(6 * 148, std::max<int64_t>(64, 65536 / experts));
+    return (int)std::min<int64_t>((rows + teams - 1) / teams, most);
+}
+template <typename T> bool whole_pieces(const void *x, int64_t stride, int64_t experts)
+{
+    return experts % kPiece<T> == 0 && stride % kPiece<T> == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
 }
 
 } // namespace
@@ -153,7 +289,7 @@ __global__ void __launch_bounds__(kWarps * 32) balance_bwd_kernel(const T *__res
 extern "C" size_t clb_balance_scratch_bytes(int64_t rows, int64_t experts)
 {
     if (rows <= 0 || experts <= 0 || experts > CLB_BALANCE_MAX_EXPERTS) return 0;
-    return (size_t)balance_blocks(rows) * (size_t)(8 * experts + 4);
+    return (size_t)balance_blocks(rows, experts) * (size_t)(8 * experts + 4);
 }
 
 extern "C" int clb_balance_fwd(const void *x, int64_t row_stride, const uint8_t *keep, float *loss, int64_t *counts, float *share, void *scratch,
@@ -166,16 +302,25 @@ extern "C" int clb_balance_fwd(const void *x, int64_t row_stride, const uint8_t 
     if (rows > 0 && !x) return CLB_ERR_ARG;
     if (rows > 0 && (!scratch || scratch_bytes < clb_balance_scratch_bytes(rows, experts))) return CLB_ERR_SCRATCH;
     cudaStream_t st = (cudaStream_t)stream;
-    const int blocks = balance_blocks(rows);
+    const int blocks = rows > 0 ? balance_blocks(rows, experts) : 0;
     float *sums = (float *)scratch;
     int *cnt = (int *)(sums + (long long)blocks * experts), *kept = cnt + (long long)blocks * experts;
     if (rows > 0)
         with_score_type(dtype, [&](auto t) {
             using T = decltype(t);
-            CLB_TRACED("balance_fwd_kernel", st,
-                       balance_fwd_kernel<T><<<blocks, kWarps * 32, 0, st>>>((const T *)x, row_stride, keep, sums, cnt, kept, rows, (int)experts, k));
+            with_team(experts, [&](auto G, auto NC) {
+                auto go = [&](auto vec) {
+                    constexpr bool VEC = decltype(vec)::value;
+                    CLB_TRACED("balance_fwd_kernel", st,
+                               balance_fwd_kernel<T, decltype(G)::value, decltype(NC)::value, VEC><<<blocks, kThreads<decltype(NC)::value>, 0, st>>>(
+                                   (const T *)x, row_stride, keep, sums, cnt, kept, (int)rows, (int)experts, k));
+                };
+                if (whole_pieces<T>(x, row_stride, experts)) go(std::true_type());
+                else go(std::false_type());
+            });
         });
-    CLB_TRACED("balance_finish_kernel", st, balance_finish_kernel<<<1, 256, 0, st>>>(sums, cnt, kept, loss, counts, share, blocks, (int)experts, k));
+    CLB_TRACED("balance_finish_kernel", st, balance_finish_kernel<<<1, 1024, 0, st>>>(sums, cnt, kept, loss, counts, share, blocks, (int)experts,
+                                                                                                  (int)(1024 / experts), k));
     return check_launch(rows > 0 ? 2 : 1);
 }
 
@@ -189,9 +334,19 @@ extern "C" int clb_balance_bwd(const void *x, int64_t row_stride, const uint8_t 
     cudaStream_t st = (cudaStream_t)stream;
     with_score_type(dtype, [&](auto t) {
         using T = decltype(t);
-        CLB_TRACED("balance_bwd_kernel", st,
-                   balance_bwd_kernel<T><<<balance_blocks(rows), kWarps * 32, 0, st>>>((const T *)x, row_stride, keep, share, upstream, (T *)grad, rows,
-                                                                                     (int)experts));
+        with_team(experts, [&](auto G, auto NC) {
+            constexpr int LANES = decltype(G)::value;
+            const int64_t teams = kThreads<decltype(NC)::value> / LANES;
+            const int blocks = (int)std::min<int64_t>((rows + teams - 1) / teams, 6 * (int64_t)sm_count());
+            auto go = [&](auto vec) {
+                constexpr bool VEC = decltype(vec)::value;
+                CLB_TRACED("balance_bwd_kernel", st,
+                           balance_bwd_kernel<T, LANES, decltype(NC)::value, VEC><<<blocks, kThreads<decltype(NC)::value>, 0, st>>>((const T *)x, row_stride, keep, share, upstream,
+                                                                                                             (T *)grad, (int)rows, (int)experts));
+            };
+            if (whole_pieces<T>(x, row_stride, experts) && (reinterpret_cast<uintptr_t>(grad) & 15) == 0) go(std::true_type());
+            else go(std::false_type());
+        });
     });
     return check_launch();
 }
