@@ -101,7 +101,8 @@ _SIGNATURES = {
     "clb_group_sum_scratch_bytes": ([_i64, _i64, _i, _i], _sz),
     "clb_group_sum_fwd": ([_vp, _vp, _vp, _sz, _i64, _i64, _i, C.c_double, _i, _vp], _i),
     "clb_group_sum_ce": ([_vp] * 6 + [_sz, _i64, _i64, _i, C.c_double, _vp], _i),
-    "clb_top_logits": ([_vp, _i64] + [_vp] * 3 + [_i64, _i64, _i, C.c_double, _i, _vp], _i),
+    "clb_top_logits_scratch_bytes": ([_i64, _i64, _i, _i], _sz),
+    "clb_top_logits": ([_vp, _i64] + [_vp] * 4 + [_sz, _i64, _i64, _i, C.c_double, _i, _vp], _i),
     "clb_distill_scratch_bytes": ([_i64, _i64, _i], _sz),
     "clb_distill_fwd": ([_vp, _i64] + [_vp] * 9 + [_sz, _i64, _i64, _i, C.c_double, _i, _i, _vp], _i),
     "clb_distill_bwd": ([_vp, _i64] + [_vp] * 4 + [_i, _i, _vp, _i64, _i64, _i, C.c_double, _i, _vp], _i),

@@ -86,6 +86,7 @@ template <typename T> struct RowPieces {
             }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
+    __device__ __forceinline__ uint4 piece(int j) const { return whole(j) ? __ldg(reinterpret_cast<const uint4 *>(row + first(j))) : edge(j); }
     // pieces j, j + step, ...: the whole ones are asked for before anything waits.  LAST: not read again
     template <int NV, bool LAST = true> __device__ __forceinline__ void load(uint4 (&q)[NV], int j, int step) const
     {
@@ -165,6 +166,29 @@ template <typename T> __device__ __forceinline__ float word_max(uint32_t w)
     float f[Word<T>::n];
     Word<T>::get(w, f);
     return fmaxf(f[0], f[Word<T>::n - 1]);
+}
+
+// the larger of two words' values, NaN above all
+template <typename T> __device__ __forceinline__ uint32_t max_nan(uint32_t a, uint32_t b);
+template <> __device__ __forceinline__ uint32_t max_nan<float>(uint32_t a, uint32_t b)
+{
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(__uint_as_float(a)), "f"(__uint_as_float(b)));
+    return __float_as_uint(r);
+}
+template <> __device__ __forceinline__ uint32_t max_nan<__half>(uint32_t a, uint32_t b) { return Word<__half>::to(__hmax2_nan(Word<__half>::of(a), Word<__half>::of(b))); }
+template <> __device__ __forceinline__ uint32_t max_nan<__nv_bfloat16>(uint32_t a, uint32_t b)
+{
+    return Word<__nv_bfloat16>::to(__hmax2_nan(Word<__nv_bfloat16>::of(a), Word<__nv_bfloat16>::of(b)));
+}
+template <typename T> __device__ __forceinline__ uint32_t piece_max_nan(const uint4 &q) { return max_nan<T>(max_nan<T>(q.x, q.y), max_nan<T>(q.z, q.w)); }
+// order_key of the larger value of such a word
+template <typename T> __device__ __forceinline__ uint32_t word_key(uint32_t w)
+{
+    float f[Word<T>::n];
+    Word<T>::get(w, f);
+    const uint32_t a = order_key(f[0]);
+    return Word<T>::n == 1 ? a : max(a, order_key(f[Word<T>::n - 1]));
 }
 
 // ---- (m, l) of exponents over lanes

@@ -1,85 +1,420 @@
 // The k largest logits of every row and the mass of the others, for losses against a teacher's lists.
 //
 // A row's classes are ordered by value, ties by index; the first k are the list, and rest = log sum over the others of exp(x / T).
-// Simple form: a block per row that looks for the next class after the last one, k times.
-#include "clb_scores.cuh"
+//
+// One read of the logits.  A team of threads (a warp for rows of up to 1024 values; a block for a segment of 8192 fp32 or 16384 half values of a longer row, so
+// that one row, too, fills part of the GPU) holds its values in registers:
+//   1. The k-th largest of the threads' own maxima, rounded down to 16 bits of its order, is a bound that at least k values reach, and few more: with 256 maxima
+//      of 64 values about 75 for k = 64.  One warp finds it by bisection.
+//   2. The values that reach the bound go to a list in shared memory; the others are added up as exponentials with respect to the bound.
+//   3. Each value's place in the list is the number of those above it; (value, index) are one 64-bit number, so that no two are alike.
+// Values that tie in great numbers, more than the list holds, take a second way: bisection over all values for the k-th largest, then over the indices of those
+// that equal it.  Segments leave their k largest and the sum of their others; a block a row puts them together.
+#include "clb_rows.cuh"
 
 using namespace clb;
 using namespace clb_host;
 
 namespace {
 
-// (order of the value, index) as one number: larger comes first in a row's list
-__device__ __forceinline__ unsigned long long place(float v, long long i) { return ((unsigned long long)order_key(v) << 32) | (0xffffffffu - (uint32_t)i); }
+typedef unsigned long long u64;
+constexpr uint32_t kMasked = 0x007fffffu; // order_key(-inf)
+constexpr int kBlock = 256;
 
-template <typename T>
-__global__ void __launch_bounds__(256) top_logits_kernel(const T *__restrict__ x, long long stride, float *__restrict__ values, int64_t *__restrict__ indices,
-                                                         float *__restrict__ rest, long long rows, int classes, int k, float temperature, float c)
+// (order of the value, index) as one number: larger comes first in a row's list; 0: nothing
+__device__ __forceinline__ u64 place_of(uint32_t key, uint32_t i) { return ((u64)key << 32) | (0xffffffffu - i); }
+__device__ __forceinline__ uint32_t index_of(u64 place) { return 0xffffffffu - (uint32_t)place; }
+__device__ __forceinline__ float value_of(uint32_t key) // of order_key
 {
-    __shared__ unsigned long long best[8];
-    __shared__ ExpSum part[8];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    for (long long r = blockIdx.x; r < rows; r += gridDim.x) {
-        const T *row = x + r * stride;
-        unsigned long long last = ~0ull;
-        for (int n = 0; n < k; ++n) {
-            unsigned long long mine = 0;
-            for (int i = threadIdx.x; i < classes; i += 256) {
-                const unsigned long long p = place(to_f(row[i]), i);
-                if (p < last && p > mine) mine = p;
-            }
-            for (int o = 16; o > 0; o >>= 1) {
-                const unsigned long long other = __shfl_xor_sync(0xffffffffu, mine, o);
-                if (other > mine) mine = other;
-            }
-            if (lane == 0) best[warp] = mine;
-            __syncthreads();
-            for (int w = 0; w < 8; ++w)
-                if (w == 0 || best[w] > mine) mine = best[w];
-            __syncthreads();
-            last = mine;
-            if (threadIdx.x == 0) {
-                const uint32_t i = 0xffffffffu - (uint32_t)last;
-                values[r * k + n] = to_f(row[i]);
-                indices[r * k + n] = i;
-            }
-        }
-        ExpSum s{-INFINITY, 0.f};
-        bool inf = false;
-        for (int i = threadIdx.x; i < classes; i += 256) {
-            const float v = to_f(row[i]);
-            if (place(v, i) >= last) continue;
-            if (v == INFINITY) inf = true;
-            else s = merge(s, single(v), c);
-        }
-        inf = __syncthreads_or(inf);
-        s = warp_merge(s, c);
-        if (lane == 0) part[warp] = s;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int w = 1; w < 8; ++w) s = merge(s, part[w], c);
-            rest[r] = inf && s.l == s.l ? INFINITY : s.m / temperature + logf(s.l);
-        }
-        __syncthreads();
+    return key == 0xfffffffeu ? __uint_as_float(0x7fc00000u) : __uint_as_float((key & 0x80000000u) ? key & 0x7fffffffu : ~key);
+}
+
+// The largest bound of 16 bits that at least k of the N * 32 keys of a warp reach (0 if k of them are 0).
+template <int N> __device__ __forceinline__ uint32_t bound_of(const uint32_t (&key)[N], int k)
+{
+    uint32_t any = key[0], all = key[0];
+#pragma unroll
+    for (int i = 1; i < N; ++i) any |= key[i], all &= key[i];
+    any = __reduce_or_sync(0xffffffffu, any), all = __reduce_and_sync(0xffffffffu, all);
+    if (!((any ^ all) >> 16)) return all & 0xffff0000u;
+    uint32_t bit = 0x80000000u >> __clz(any ^ all); // (what is above is the same in all keys)
+    uint32_t bound = all & ~(2 * bit - 1);
+#pragma unroll 1
+    for (; bit >= 0x10000u; bit >>= 1) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < N; ++i) n += key[i] >= (bound | bit);
+        if (__reduce_add_sync(0xffffffffu, n) >= k) bound |= bit;
     }
+    return bound;
+}
+
+struct TopArgs {
+    long long stride, rows;
+    int classes, k, segments;
+    float temperature, c; // c = log2(e) / T
+};
+
+// Counts, flags and sums over a team of TH threads: of a warp, or of the block through `box` (TH / 32 + 1 words).
+template <int TH> __device__ __forceinline__ void team_sync()
+{
+    if (TH == 32) __syncwarp();
+    else __syncthreads();
+}
+template <int TH> __device__ __forceinline__ int team_count(int n, int *box)
+{
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (TH == 32) return n;
+    if ((threadIdx.x & 31) == 0) box[threadIdx.x >> 5] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < TH / 32; ++w) n += box[w];
+    __syncthreads();
+    return n;
+}
+template <int TH> __device__ __forceinline__ ExpSum team_merge(ExpSum s, ExpSum *box, float c)
+{
+    s = lanes_merge<32>(s, c);
+    if (TH == 32) return s;
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) box[threadIdx.x >> 5] = s;
+    __syncthreads();
+    return lanes_merge<TH / 32>(box[threadIdx.x % (TH / 32)], c);
+}
+
+// the place of each of `count` candidates among them, handed to `f`
+template <int TH, typename F> __device__ __forceinline__ void ranked(const u64 *cand, int count, int t, F &&f)
+{
+    for (int i = t; i < count; i += TH) {
+        const u64 mine = cand[i];
+        int above = 0;
+#pragma unroll 4
+        for (int j = 0; j < count; j += 2) { // (the list is padded with a 0)
+            const ulonglong2 two = *reinterpret_cast<const ulonglong2 *>(cand + j);
+            above += (two.x > mine) + (two.y > mine);
+        }
+        f(above, mine);
+    }
+}
+
+// TH threads a row (32) or a segment of one (256), NV pieces a thread.
+template <typename T, int TH, int NV>
+__global__ void __launch_bounds__(kBlock, 4) top_select_kernel(const T *__restrict__ x, float *__restrict__ values, int64_t *__restrict__ indices,
+                                                               float *__restrict__ rest, u64 *__restrict__ places, ExpSum *__restrict__ sums, TopArgs a)
+{
+    constexpr int TEAMS = kBlock / TH, EV = kPiece<T>, SUB = TH == 32 ? 4 : 1, CAP = TH == 32 ? 256 : 512;
+    static_assert(NV % SUB == 0, "groups of whole pieces");
+    __shared__ __align__(16) u64 cand_all[TEAMS][CAP + 2];
+    __shared__ uint32_t keys_all[TEAMS][TH * SUB], extra_all[TEAMS][CAP];
+    __shared__ int count_all[TEAMS], box[TH / 32 + 1];
+    __shared__ uint32_t bound_all[TEAMS];
+    __shared__ ExpSum sum_box[TH / 32];
+    const int t = threadIdx.x % TH, team = threadIdx.x / TH;
+    u64 *const cand = cand_all[team];
+    const long long items = a.rows * a.segments;
+    for (long long item = (long long)blockIdx.x * TEAMS + team; item < items; item += (long long)gridDim.x * TEAMS) {
+        const long long r = a.segments == 1 ? item : item / a.segments;
+        const int seg = a.segments == 1 ? 0 : (int)(item - r * a.segments);
+        const RowPieces<T> row(x + r * a.stride, a.classes);
+        const int base = seg * TH * NV;
+        uint4 raw[NV];
+        row.load(raw, base + t, TH);
+        // the class of value e of the thread's piece i, -1 for none
+        auto class_of = [&](int i, int e) {
+            const int c = row.first(base + i * TH + t) + e;
+            return c >= 0 && c < a.classes ? c : -1;
+        };
+        auto value_at = [&](int i, int e) {
+            const uint32_t w = (&raw[i].x)[sizeof(T) == 4 ? e & 3 : e >> 1];
+            float f[Word<T>::n];
+            Word<T>::get(w, f);
+            return f[Word<T>::n == 1 ? 0 : e & 1];
+        };
+        // ---- 1: the bound
+        uint32_t tops[NV];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) tops[i] = piece_max_nan<T>(raw[i]);
+#pragma unroll
+        for (int s = 0; s < SUB; ++s) {
+            uint32_t top = tops[s * (NV / SUB)];
+#pragma unroll
+            for (int i = 1; i < NV / SUB; ++i) top = max_nan<T>(top, tops[s * (NV / SUB) + i]);
+            keys_all[team][s * TH + t] = word_key<T>(top);
+        }
+        if (t == 0) count_all[team] = 0;
+        team_sync<TH>();
+        if (t < 32) {
+            uint32_t key[TH * SUB / 32];
+#pragma unroll
+            for (int i = 0; i < TH * SUB / 32; ++i) key[i] = keys_all[team][i * 32 + t];
+            const uint32_t b = bound_of(key, a.k);
+            // (fewer than k groups have a value: all values are candidates, and the first k of the masked)
+            if (t == 0) bound_all[team] = b <= kMasked ? kMasked + 1 : b;
+        }
+        team_sync<TH>();
+        const uint32_t bound = bound_all[team];
+        const bool few = bound == kMasked + 1;
+        const float reach = value_of(bound);
+        // ---- 2: candidates, and the sum of the others
+        auto push = [&](float v, int cls) {
+            const int n = atomicAdd(&count_all[team], 1);
+            if (n < CAP) cand[n] = place_of(order_key(v), cls);
+        };
+        const int first_class = max(0, row.first(base));
+        const int own_first = base == 0 ? 0 : first_class; // the segment's first class
+        const ExpRef er = exp_ref(reach, a.c);
+        float l = 0.f;
+        uint32_t hits = 0; // pieces with a candidate
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            float f[Word<T>::n];
+            Word<T>::get(tops[i], f);
+            const bool hit = !(f[0] < reach) || !(f[Word<T>::n - 1] < reach) || (few && row.first(base + i * TH + t) < own_first + a.k);
+            hits |= (uint32_t)hit << i;
+            const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                float g[Word<T>::n];
+                Word<T>::get(w[q], g);
+#pragma unroll
+                for (int z = 0; z < Word<T>::n; ++z)
+                    if (g[z] < reach) l += ex2(fmaf(g[z], a.c, -er.R));
+            }
+        }
+        while (hits) { // read once more: a warp has as many turns as its lanes have such pieces at most, one or two, not one for every piece
+            const int i = __ffs(hits) - 1;
+            hits &= hits - 1;
+            const uint4 p = row.piece(base + i * TH + t);
+            const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+            for (int e = 0; e < EV; ++e) {
+                float f[Word<T>::n];
+                Word<T>::get(w[Word<T>::n == 1 ? e & 3 : e >> 1], f);
+                const float v = f[Word<T>::n == 1 ? 0 : e & 1];
+                const int cls = class_of(i, e);
+                if (cls >= 0 && (!(v < reach) || (few && cls < own_first + a.k))) push(v, cls);
+            }
+        }
+        l *= er.fix;
+        team_sync<TH>();
+        int count = count_all[team];
+        // f(value, class) for each of the thread's values; code of its own, as what follows is rare (a rotation: no register is named by a number that varies)
+        auto for_each = [&](auto f) {
+#pragma unroll 1
+            for (int i = 0; i < NV; ++i) {
+                const uint4 q = raw[0];
+#pragma unroll
+                for (int n = 1; n < NV; ++n) raw[n - 1] = raw[n];
+                raw[NV - 1] = q;
+#pragma unroll
+                for (int e = 0; e < EV; ++e)
+                    if (class_of(i, e) >= 0) f(value_at(NV - 1, e), class_of(i, e));
+            }
+        };
+        const bool overflow = count > CAP;
+        if (overflow) { // ---- the k-th largest key, then the last index of those that equal it
+            uint32_t key = 0, last = 0;
+            int n;
+            for (uint32_t bit = 0x80000000u; bit; bit >>= 1) {
+                n = 0;
+                for_each([&](float v, int) { n += order_key(v) >= (key | bit); });
+                if (team_count<TH>(n, box) >= a.k) key |= bit;
+            }
+            n = 0;
+            for_each([&](float v, int) { n += order_key(v) > key; });
+            const int need = a.k - team_count<TH>(n, box);
+            for (uint32_t bit = 1u << 30; bit; bit >>= 1) { // the largest class that fewer than `need` of them are below
+                n = 0;
+                for_each([&](float v, int cls) { n += (uint32_t)cls < (last | bit) && order_key(v) == key; });
+                if (team_count<TH>(n, box) < need) last |= bit;
+            }
+            if (t == 0) count_all[team] = 0;
+            team_sync<TH>();
+            for_each([&](float v, int cls) {
+                if (order_key(v) > key || (order_key(v) == key && (uint32_t)cls <= last)) push(v, cls);
+            });
+            team_sync<TH>();
+            count = count_all[team];
+        }
+        if (t == 0) cand[count] = cand[count + 1] = 0;
+        team_sync<TH>();
+        // ---- 3: their places
+        ExpSum others{reach, l};
+        bool inf = false;
+        const long long at = item * a.k;
+        uint32_t *const kth_box = keys_all[team];
+        ranked<TH>(cand, count, t, [&](int rank, u64 place) {
+            const uint32_t key = (uint32_t)(place >> 32);
+            if (rank < a.k) {
+                if (a.segments == 1) values[at + rank] = value_of(key), indices[at + rank] = index_of(place);
+                else places[at + rank] = place;
+                if (rank == a.k - 1) kth_box[0] = key, kth_box[1] = (uint32_t)place;
+            } else
+                extra_all[team][rank - a.k] = key;
+        });
+        team_sync<TH>();
+        for (int i = t; i < count - a.k; i += TH) { // in the order of their places, whatever the order in which they came to the list
+            const float v = value_of(extra_all[team][i]);
+            if (v == INFINITY) inf = true;
+            else others = merge(others, single(v), a.c);
+        }
+        if (a.segments > 1)
+            for (int n = count + t; n < a.k; n += TH) places[at + n] = 0; // a last segment of few classes
+        others = team_merge<TH>(others, sum_box, a.c);
+        if (overflow || er.far || !(reach < INFINITY) || !(others.l > 1e-20f)) {
+            // the bound is no reference for the others, or they are not all counted: once more, with respect to their own largest
+            const u64 kth = count >= a.k ? ((u64)kth_box[0] << 32) | kth_box[1] : 0;
+            others = ExpSum{-INFINITY, 0.f}, inf = false;
+            for_each([&](float v, int cls) {
+                if (place_of(order_key(v), cls) >= kth) return;
+                if (v == INFINITY) inf = true;
+                else others = merge(others, single(v), a.c);
+            });
+            others = team_merge<TH>(others, sum_box, a.c);
+        }
+        if (team_count<TH>(inf, box) && others.l == others.l) others = ExpSum{INFINITY, 1.f};
+        if (t == 0) {
+            if (a.segments == 1) rest[r] = others.m / a.temperature + logf(others.l);
+            else sums[item] = others;
+        }
+        team_sync<TH>(); // the tables are used again
+    }
+}
+
+// A row's segments put together: a block a row.  places [rows][segments * k], sums [rows][segments].
+__global__ void __launch_bounds__(kBlock) top_merge_kernel(const u64 *__restrict__ places, const ExpSum *__restrict__ sums, float *__restrict__ values,
+                                                           int64_t *__restrict__ indices, float *__restrict__ rest, TopArgs a)
+{
+    constexpr int CAP = 512, WARPS = kBlock / 32;
+    __shared__ __align__(16) u64 cand[CAP + 2];
+    __shared__ uint32_t keys[kBlock], bound_box;
+    __shared__ int count_box, box[WARPS];
+    __shared__ u64 kth_box, best[WARPS];
+    __shared__ ExpSum sum_box[WARPS];
+    const int t = threadIdx.x, n = a.segments * a.k;
+    for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
+        const u64 *p = places + r * n;
+        uint32_t top = 0;
+        for (int i = t; i < n; i += kBlock) top = max(top, (uint32_t)(p[i] >> 32));
+        keys[t] = top;
+        if (t == 0) count_box = 0;
+        __syncthreads();
+        if (t < 32) {
+            uint32_t key[WARPS];
+#pragma unroll
+            for (int i = 0; i < WARPS; ++i) key[i] = keys[i * 32 + t];
+            const uint32_t b = bound_of(key, a.k);
+            if (t == 0) bound_box = b;
+        }
+        __syncthreads();
+        const uint32_t bound = max(bound_box, 1u); // (0: no value)
+        for (int i = t; i < n; i += kBlock)
+            if ((uint32_t)(p[i] >> 32) >= bound) {
+                const int c = atomicAdd(&count_box, 1);
+                if (c < CAP) cand[c] = p[i];
+            }
+        __syncthreads();
+        const int count = count_box;
+        if (count <= CAP) {
+            if (t == 0) cand[count] = cand[count + 1] = 0;
+            __syncthreads();
+            ranked<kBlock>(cand, count, t, [&](int rank, u64 place) {
+                if (rank >= a.k) return;
+                values[r * a.k + rank] = value_of((uint32_t)(place >> 32)), indices[r * a.k + rank] = index_of(place);
+                if (rank == a.k - 1) kth_box = place;
+            });
+        } else { // values that tie in great numbers: the next one after the last, k times
+            u64 last = ~0ull;
+            for (int i = 0; i < a.k; ++i) {
+                u64 mine = 0;
+                for (int j = t; j < n; j += kBlock)
+                    if (p[j] < last && p[j] > mine) mine = p[j];
+#pragma unroll
+                for (int o = 16; o > 0; o >>= 1) mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, o));
+                if ((t & 31) == 0) best[t >> 5] = mine;
+                __syncthreads();
+                last = 0;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) last = max(last, best[w]);
+                if (t == 0) values[r * a.k + i] = value_of((uint32_t)(last >> 32)), indices[r * a.k + i] = index_of(last);
+                __syncthreads();
+            }
+            if (t == 0) kth_box = last;
+        }
+        __syncthreads();
+        const u64 kth = kth_box;
+        ExpSum others{-INFINITY, 0.f};
+        bool inf = false;
+        auto add = [&](ExpSum s) {
+            if (s.m == INFINITY) inf = true;
+            else others = merge(others, s, a.c);
+        };
+        for (int i = t; i < n; i += kBlock)
+            if (p[i] && p[i] < kth) add(single(value_of((uint32_t)(p[i] >> 32))));
+        for (int i = t; i < a.segments; i += kBlock) add(sums[r * a.segments + i]);
+        others = team_merge<kBlock>(others, sum_box, a.c);
+        if (team_count<kBlock>(inf, box) && others.l == others.l) others = ExpSum{INFINITY, 1.f};
+        if (t == 0) rest[r] = others.m / a.temperature + logf(others.l);
+        __syncthreads(); // the tables are used again
+    }
+}
+
+constexpr int kWarpPieces(int size) { return size == 4 ? 8 : 4; } // 32 values a lane
+constexpr int kSegmentPieces = 8;                                 // 32 KB a block
+
+// pieces of the longest row (rows at a multiple of 16 bytes all begin at the first one's place in its piece; with `any`, at the worst)
+template <typename T> long long most_pieces(const void *x, int64_t stride, int64_t rows, int64_t classes, bool any = false)
+{
+    const int phase = !any && (rows == 1 || stride % kPiece<T> == 0) ? (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) : kPiece<T> - 1;
+    return (classes + phase + kPiece<T> - 1) / kPiece<T>;
+}
+template <typename T> int segments_of(long long pieces)
+{
+    return pieces <= 32 * kWarpPieces(sizeof(T)) ? 1 : (int)((pieces + kBlock * kSegmentPieces - 1) / (kBlock * kSegmentPieces));
 }
 
 } // namespace
 
-extern "C" int clb_top_logits(const void *x, int64_t row_stride, float *values, int64_t *indices, float *rest, int64_t rows, int64_t classes, int k,
-                              double temperature, int dtype, void *stream)
+extern "C" size_t clb_top_logits_scratch_bytes(int64_t rows, int64_t classes, int k, int dtype)
 {
-    if (!x || !values || !indices || !rest || rows < 0 || classes <= 0 || row_stride < 0 || k <= 0 || !(temperature >= 1e-30 && temperature <= 1e30)) return CLB_ERR_ARG;
+    if (rows <= 0 || classes <= 0 || k <= 0 || classes > CLB_CLASSES_MAX) return 0;
+    int segments = 0;
+    with_score_type(dtype, [&](auto t) { segments = segments_of<decltype(t)>(most_pieces<decltype(t)>(nullptr, 1, rows, classes, true)); });
+    return segments > 1 ? (size_t)rows * segments * (8 * (size_t)k + sizeof(ExpSum)) : 0;
+}
+
+extern "C" int clb_top_logits(const void *x, int64_t row_stride, float *values, int64_t *indices, float *rest, void *scratch, size_t scratch_bytes, int64_t rows,
+                              int64_t classes, int k, double temperature, int dtype, void *stream)
+{
+    if (!x || !values || !indices || !rest || rows < 0 || classes <= 0 || row_stride < 0 || k <= 0 || !(temperature >= 1e-30 && temperature <= 1e30))
+        return CLB_ERR_ARG;
     if (k > classes) return CLB_ERR_SHAPE;
     if (k > CLB_TOP_MAX || classes > CLB_CLASSES_MAX) return CLB_ERR_TOO_LARGE;
     if (dtype != CLB_F32 && dtype != CLB_F16 && dtype != CLB_BF16) return CLB_ERR_ARG;
     if (rows == 0) return CLB_OK;
+    if (scratch_bytes < clb_top_logits_scratch_bytes(rows, classes, k, dtype) || (!scratch && clb_top_logits_scratch_bytes(rows, classes, k, dtype)))
+        return CLB_ERR_SCRATCH;
     cudaStream_t st = (cudaStream_t)stream;
-    with_score_type(dtype, [&](auto t) {
-        using T = decltype(t);
-        CLB_TRACED("top_logits_kernel", st,
-                   top_logits_kernel<T><<<(unsigned)(rows < (1 << 20) ? rows : (1 << 20)), 256, 0, st>>>(
-                       (const T *)x, row_stride, values, indices, rest, rows, (int)classes, k, (float)temperature, (float)(1.4426950408889634 / temperature)));
+    int launches = 1;
+    with_score_type(dtype, [&](auto v) {
+        using T = decltype(v);
+        const long long pieces = most_pieces<T>(x, row_stride, rows, classes);
+        TopArgs a{row_stride, rows, (int)classes, k, segments_of<T>(pieces), (float)temperature, (float)(1.4426950408889634 / temperature)};
+        u64 *const places = (u64 *)scratch;
+        ExpSum *const sums = (ExpSum *)(places + (a.segments > 1 ? rows * a.segments * k : 0));
+        auto blocks = [](long long n) { return (unsigned)(n < (1 << 20) ? n : (1 << 20)); };
+        if (pieces <= 32 * kWarpPieces(sizeof(T))) {
+            CLB_TRACED("top_select_kernel", st,
+                       top_select_kernel<T, 32, kWarpPieces(sizeof(T))><<<blocks((rows + 7) / 8), kBlock, 0, st>>>((const T *)x, values, indices, rest, places, sums, a));
+            return;
+        }
+        CLB_TRACED("top_select_kernel", st,
+                   top_select_kernel<T, kBlock, kSegmentPieces><<<blocks(rows * a.segments), kBlock, 0, st>>>((const T *)x, values, indices, rest, places, sums, a));
+        if (a.segments > 1) {
+            CLB_TRACED("top_merge_kernel", st, top_merge_kernel<<<blocks(rows), kBlock, 0, st>>>(places, sums, values, indices, rest, a));
+            launches = 2;
+        }
     });
-    return check_launch();
+    return check_launch(launches);
 }

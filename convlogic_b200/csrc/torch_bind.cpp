@@ -1054,8 +1054,10 @@ std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor &x_in, int64_t k, dou
     check_top(k, x.classes);
     Below below(x.x);
     Tensor values = alloc(row_shape(x_in, k), x.x, at::kFloat), indices = alloc(row_shape(x_in, k), x.x, at::kLong), rest = alloc(row_shape(x_in), x.x, at::kFloat);
+    const size_t bytes = clb_top_logits_scratch_bytes(x.rows, x.classes, (int)k, x.dtype);
+    Tensor scratch = scratch_bytes(bytes, x.x);
     if (x.rows)
-        check(clb_top_logits(ptr(x.x), x.stride, ptr<float>(values), ptr<int64_t>(indices), ptr<float>(rest), x.rows, x.classes, (int)k, temperature, x.dtype,
+        check(clb_top_logits(ptr(x.x), x.stride, ptr<float>(values), ptr<int64_t>(indices), ptr<float>(rest), ptr(scratch), bytes, x.rows, x.classes, (int)k, temperature, x.dtype,
                              cur_stream()));
     return {values, indices, rest};
 }

@@ -425,11 +425,13 @@ int clb_group_sum_ce(const float *y, const int64_t *labels, float *scores, float
  *
  * clb_top_logits: per row the k largest of `classes` logits, values [rows][k] in descending order, indices int64 [rows][k]; equal
  * values by index, NaN before every number.  rest [rows] = log of the sum of exp(x / temperature) over the classes that are not listed, -inf where
- * there is none.  1 <= k <= min(classes, CLB_TOP_MAX), temperature from 1e-30 to 1e30. */
+ * there is none.  1 <= k <= min(classes, CLB_TOP_MAX), temperature from 1e-30 to 1e30.  scratch:
+ * clb_top_logits_scratch_bytes (0 for short rows), 16-byte aligned. */
 #define CLB_TOP_MAX 128
 #define CLB_CLASSES_MAX (1 << 30)
-int clb_top_logits(const void *x, int64_t row_stride, float *values, int64_t *indices, float *rest, int64_t rows, int64_t classes, int k,
-                   double temperature, int dtype, void *stream);
+size_t clb_top_logits_scratch_bytes(int64_t rows, int64_t classes, int k, int dtype);
+int clb_top_logits(const void *x, int64_t row_stride, float *values, int64_t *indices, float *rest, void *scratch, size_t scratch_bytes, int64_t rows,
+                   int64_t classes, int k, double temperature, int dtype, void *stream);
 
 /* Loss of scores against a teacher's lists, temperature^2 KL(teacher || student) with all classes outside a row's list taken as one:
  *   p, r = soft-max over (values / temperature, rest), q = softmax(scores / temperature), q_r = sum of q over the unlisted classes,

@@ -27,17 +27,18 @@ def test_names():
 
 def test_bad_arguments_are_refused_before_any_launch(lib):
     p = 1 << 20   # never looked at
-    args = dict(x=p, stride=10, values=p, indices=p, rest=p, rows=4, classes=10, k=3, t=1.0, dtype=0)
+    args = dict(x=p, stride=10, values=p, indices=p, rest=p, rows=4, classes=10, k=3, t=1.0, dtype=0, scratch=p, size=0)
 
     def top(**kw):
         a = {**args, **kw}
-        return lib.clb_top_logits(a["x"], a["stride"], a["values"], a["indices"], a["rest"], a["rows"], a["classes"], a["k"], a["t"], a["dtype"], None)
+        return lib.clb_top_logits(a["x"], a["stride"], a["values"], a["indices"], a["rest"], a["scratch"], a["size"], a["rows"], a["classes"], a["k"], a["t"], a["dtype"], None)
 
     for kw, want in (({"x": None}, -1), ({"values": None}, -1), ({"rest": None}, -1), ({"rows": -1}, -1), ({"classes": 0}, -1), ({"stride": -1}, -1), ({"k": 0}, -1),
                      ({"t": 0.0}, -1), ({"t": float("nan")}, -1), ({"t": -1.0}, -1), ({"dtype": 1}, -1), ({"dtype": 7}, -1), ({"k": 11}, -2),
                      ({"k": 129, "classes": 1000}, -6), ({"classes": 1 << 31}, -6)):
         assert top(**kw) == want, kw
-    assert top(rows=0) == 0
+    assert top(rows=0) == 0 and top(classes=100000, scratch=None) == -4 and top(classes=100000, size=100) == -4
+    assert lib.clb_top_logits_scratch_bytes(4, 10, 3, 0) == 0 and lib.clb_top_logits_scratch_bytes(4, 100000, 3, 0) >= 4 * 13 * 32
 
     def fwd(loss=p, stats=p, listed=p, scratch=p, size=1 << 20, rows=4, classes=10, k=3, t=1.0, how=1, dtype=0, scores=p):
         return lib.clb_distill_fwd(scores, 10, p, p, None, None, loss, stats, listed, None, scratch, size, rows, classes, k, t, how, dtype, None)
