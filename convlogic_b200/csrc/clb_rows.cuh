@@ -18,6 +18,42 @@ __device__ __forceinline__ float ex2(float v)
     return r;
 }
 
+// Two floats at once: one instruction for two sums, products or fused multiply-adds.
+struct Pair {
+    unsigned long long v;
+};
+__device__ __forceinline__ Pair pair_of(float a, float b)
+{
+    Pair p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p.v) : "f"(a), "f"(b));
+    return p;
+}
+__device__ __forceinline__ void split(Pair p, float &a, float &b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(p.v)); }
+__device__ __forceinline__ Pair operator+(Pair a, Pair b)
+{
+    Pair p;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+    return p;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b)
+{
+    Pair p;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(p.v) : "l"(a.v), "l"(b.v));
+    return p;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c)
+{
+    Pair p;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(p.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return p;
+}
+__device__ __forceinline__ Pair ex2(Pair p)
+{
+    float a, b;
+    split(p, a, b);
+    return pair_of(ex2(a), ex2(b));
+}
+
 template <typename T> constexpr int kPiece = 16 / (int)sizeof(T); // values of a piece
 template <typename T> __device__ __forceinline__ constexpr uint32_t low_bits() { return sizeof(T) == 4 ? 0xff800000u : 0u; }
 template <> __device__ __forceinline__ constexpr uint32_t low_bits<__half>() { return 0xfc00u; }
@@ -56,6 +92,17 @@ template <> struct Word<__nv_bfloat16> {
     static __device__ __forceinline__ uint32_t put(const float (&v)[2]) { return to(__floats2bfloat162_rn(v[0], v[1])); }
     static __device__ __forceinline__ uint32_t max(uint32_t a, uint32_t b) { return to(__hmax2(of(a), of(b))); }
 };
+
+// (as function templates: the float case has one value a word, and never calls them)
+template <typename T> __device__ __forceinline__ void two_values(uint32_t w, float (&f)[2])
+{
+    if constexpr (sizeof(T) == 2) Word<T>::get(w, f);
+}
+template <typename T> __device__ __forceinline__ uint32_t two_word(const float (&f)[2])
+{
+    if constexpr (sizeof(T) == 2) return Word<T>::put(f);
+    return 0;
+}
 
 // where the pieces of a row lie
 template <typename T> struct RowPieces {
@@ -107,7 +154,7 @@ template <typename T> struct RowPieces {
         }
         if (j == 0 && !whole(0)) q[0] = edge(0); // (a first piece is some thread's first)
         const int last = pieces - 1, i = last - j;
-        if (last > 0 && i >= 0 && i < NV * step && (i & (step - 1)) == 0 && !whole(last)) { // (step: a power of two)
+        if (last > 0 && i >= 0 && i < NV * step && i % step == 0 && !whole(last)) {
             const uint4 e = edge(last);
 #pragma unroll
             for (int n = 0; n < NV; ++n) {
@@ -145,17 +192,51 @@ template <typename T> __device__ __forceinline__ void drop_value(uint4 &q, int e
     else w[e >> 1] = (e & 1) ? (w[e >> 1] & 0xffffu) | low_bits<T>() << 16 : (w[e >> 1] & 0xffff0000u) | low_bits<T>();
     q = make_uint4(w[0], w[1], w[2], w[3]);
 }
-// sum of the exponentials of a piece's values with respect to R / c, in two chains
-template <typename T> __device__ __forceinline__ void piece_exp_sum(float (&l)[2], const uint4 &p, float R, float c)
+// a piece's values in pairs
+template <typename T> constexpr int kPairs = kPiece<T> / 2;
+template <typename T> __device__ __forceinline__ void piece_pairs(const uint4 &p, Pair (&v)[kPairs<T>])
 {
     const uint32_t w[4] = {p.x, p.y, p.z, p.w};
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        float f[Word<T>::n];
-        Word<T>::get(w[q], f);
-#pragma unroll
-        for (int z = 0; z < Word<T>::n; ++z) l[(q + z) & 1] += ex2(fmaf(f[z], c, -R));
+    for (int i = 0; i < kPairs<T>; ++i) {
+        if (sizeof(T) == 4) v[i] = pair_of(__uint_as_float(w[2 * i & 3]), __uint_as_float(w[2 * i + 1 & 3]));
+        else {
+            float f[2];
+            two_values<T>(w[i & 3], f);
+            v[i] = pair_of(f[0], f[1]);
+        }
     }
+}
+template <typename T> __device__ __forceinline__ uint4 pairs_piece(const Pair (&v)[kPairs<T>])
+{
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < kPairs<T>; ++i) {
+        float f[2];
+        split(v[i], f[0], f[1]);
+        if (sizeof(T) == 4) w[2 * i & 3] = __float_as_uint(f[0]), w[2 * i + 1 & 3] = __float_as_uint(f[1]);
+        else w[i & 3] = two_word<T>(f);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+// adds the exponentials of a piece's values with respect to R / c
+template <typename T> __device__ __forceinline__ void piece_exp_sum(Pair (&l)[2], const uint4 &p, Pair minus_R, Pair c)
+{
+    Pair v[kPairs<T>];
+    piece_pairs<T>(p, v);
+#pragma unroll
+    for (int i = 0; i < kPairs<T>; ++i) l[i & 1] = l[i & 1] + ex2(fma2(v[i], c, minus_R));
+}
+// the classes whose bits are set become -inf
+template <typename T> __device__ __forceinline__ void strike_out(uint4 *q, uint32_t bits, int pieces)
+{
+    if (bits)
+#pragma unroll
+        for (int i = 0; i < pieces; ++i)
+            if ((bits >> (i * kPiece<T>)) & ((1u << kPiece<T>) - 1))
+#pragma unroll
+                for (int e = 0; e < kPiece<T>; ++e)
+                    if ((bits >> (i * kPiece<T> + e)) & 1) drop_value<T>(q[i], e);
 }
 template <typename T> __device__ __forceinline__ uint32_t piece_max(uint32_t top, const uint4 &q)
 {
@@ -205,8 +286,13 @@ __device__ __forceinline__ ExpRef exp_ref(float m, float c)
     r.R = m * c, r.far = !(fabsf(m) < 1e38f && fabsf(r.R) < 1e38f), r.fix = ex2(-fmaf(m, c, -r.R));
     return r;
 }
-template <int LANES> __device__ __forceinline__ float lanes_max(float v)
+template <int LANES> __device__ __forceinline__ float lanes_max(float v) // NaN is passed over
 {
+    if (LANES == 32) { // one instruction for the warp
+        float r;
+        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+        return r;
+    }
 #pragma unroll
     for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
     return v;
@@ -223,5 +309,21 @@ template <int LANES> __device__ __forceinline__ ExpSum lanes_merge(ExpSum s, flo
     const float m = lanes_max<LANES>(s.m);
     return {m, lanes_sum<LANES>(s.l * exp_of(s.m, finite_or_zero(m), c))};
 }
+
+// A row cut into trips of TH * NV pieces: those from `lo` on and below `hi` are whole, whichever thread asks.
+template <typename T, int TH, int NV> struct RowTrips {
+    static constexpr int kBytes = TH * NV * 16;
+    const char *first; // the thread's piece 0 of trip 0 (not to be read unless trip 0 is whole)
+    int lo, hi;
+    __device__ __forceinline__ RowTrips() = default;
+    __device__ __forceinline__ RowTrips(const T *row, int classes)
+    {
+        const int phase = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));
+        first = reinterpret_cast<const char *>(row) - phase * (int)sizeof(T) + threadIdx.x * 16;
+        lo = phase ? 1 : 0, hi = (int)(((long long)classes + phase) / (kBytes / (int)sizeof(T)));
+    }
+    __device__ __forceinline__ bool whole(int trip) const { return trip >= lo && trip < hi; }
+    __device__ __forceinline__ const char *at(int trip) const { return first + (long long)trip * kBytes; }
+};
 
 } // namespace clb

@@ -33,35 +33,43 @@ struct Entry { // one class of a list: cls < 0: does not exist
     float t, s;
 };
 
-// What a row's sums come to: unlisted scores `rest`, distinct listed ones `list`, the teacher's listed values `teach`, the teacher's rest rs, the weight.
+// What a teacher's list comes to: its listed values' sum, its rest rs, the row's weight.
+struct TeacherNumbers {
+    float tm, tl;   // its mass is tl * exp(tm)
+    float rest;     // probability of the rest
+    float factor;   // of the row's loss / T and gradient; 0: the row adds nothing
+};
+__device__ __forceinline__ TeacherNumbers teacher_numbers(ExpSum teach, float rs, float w, const DistillArgs &a)
+{
+    TeacherNumbers q;
+    const float tz = teach.m == -INFINITY ? -INFINITY : teach.m / a.temperature;
+    q.tm = finite_or_zero(fmaxf(tz, rs));
+    const float re = ex2((rs - q.tm) * 1.44269504f);
+    q.tl = (teach.m == -INFINITY ? teach.l : teach.l * ex2((tz - q.tm) * 1.44269504f)) + re;
+    q.rest = re / q.tl;
+    q.factor = q.tl != 0.f ? w * a.scale : 0.f;
+    return q;
+}
+// What a row's sums come to: unlisted scores `rest`, distinct listed ones `list`.
 struct RowNumbers {
-    float m, coef, factor;              // unlisted gradient = coef * exp((s - m) / T); the list's = factor * (q - p)
-    float um, ul, tm, tl, re, log_rest; // all scores; the teacher's mass, exp(rest - tm); log of the unlisted scores' sum over ul's
-    bool there;
-    __device__ __forceinline__ float log_p(float t, float tt) const { return (t / tt - tm) - logf(tl); }
-    __device__ __forceinline__ float log_q(float s, float tt) const { return (s - um) / tt - logf(ul); }
-    __device__ __forceinline__ float loss(float listed, float rs, float tt) const
+    float m, l, coef;  // of the unlisted scores: reference and sum; gradient = coef * exp((s - m) / T).  The list's = factor * (q - p)
+    float um, ul;      // of all scores; ul = 0: there are none
+    __device__ __forceinline__ float loss(float listed, const TeacherNumbers &q, float rs, float tt) const // listed: the list's terms
     {
-        const float r = re / tl;
-        if (r > 0.f || r != r) listed += r * (((rs - tm) - logf(tl)) - log_rest);
-        return there ? listed * factor * tt : 0.f;
+        if (q.rest > 0.f || q.rest != q.rest) {
+            const float log_q = l == 0.f ? -INFINITY : ((m - um) / tt + logf(l)) - logf(ul);
+            listed += q.rest * (((rs - q.tm) - logf(q.tl)) - log_q);
+        }
+        return listed * q.factor * tt;
     }
 };
-__device__ __forceinline__ RowNumbers row_numbers(ExpSum rest, ExpSum list, ExpSum teach, float rs, float w, const DistillArgs &a)
+__device__ __forceinline__ RowNumbers row_numbers(ExpSum rest, ExpSum list, const TeacherNumbers &q, const DistillArgs &a)
 {
-    RowNumbers n;
-    const bool no_rest = rest.m == -INFINITY && rest.l == 0.f, no_list = list.m == -INFINITY && list.l == 0.f;
-    n.m = finite_or_zero(rest.m), n.um = finite_or_zero(fmaxf(rest.m, list.m));
-    const float of_rest = no_rest ? 0.f : rest.l * exp_of(n.m, n.um, a.c);
-    n.ul = of_rest + (no_list ? 0.f : list.l * exp_of(finite_or_zero(list.m), n.um, a.c));
-    const float tz = teach.m == -INFINITY ? -INFINITY : teach.m / a.temperature;
-    n.tm = finite_or_zero(fmaxf(tz, rs));
-    n.re = ex2((rs - n.tm) * 1.44269504f);
-    n.tl = (teach.m == -INFINITY ? teach.l : teach.l * ex2((tz - n.tm) * 1.44269504f)) + n.re;
-    n.there = w != 0.f && n.tl != 0.f && !(no_rest && no_list);
-    n.factor = w * a.scale;
-    n.coef = n.there && !no_rest ? n.factor * (__fdividef(of_rest, n.ul) - __fdividef(n.re, n.tl)) / rest.l : 0.f;
-    n.log_rest = no_rest ? -INFINITY : (n.m - n.um) / a.temperature + logf(rest.l) - logf(n.ul);
+    RowNumbers n; // (a sum of 0 has no terms: the largest adds 1)
+    n.m = finite_or_zero(rest.m), n.um = finite_or_zero(fmaxf(rest.m, list.m)), n.l = rest.l;
+    const float of_rest = rest.l == 0.f ? 0.f : rest.l * exp_of(n.m, n.um, a.c);
+    n.ul = of_rest + (list.l == 0.f ? 0.f : list.l * exp_of(finite_or_zero(list.m), n.um, a.c));
+    n.coef = q.factor == 0.f || rest.l == 0.f ? 0.f : q.factor * __fdividef(__fdividef(of_rest, n.ul) - q.rest, rest.l);
     return n;
 }
 
@@ -73,7 +81,7 @@ constexpr int kValues = 64; // of a row in a thread's registers, as fp32
 // A thread takes the exponentials of its values with respect to its own maximum and keeps them, so that there is one exchange in the team, of pairs (maximum,
 // sum), and the gradient is the kept exponential times a factor of the thread's: one exponential a value.
 template <typename T, int TH, int NV, bool CLUSTER>
-__global__ void __launch_bounds__(TH <= 32 ? 256 : TH, TH <= 32 ? 2 : 512 / TH)
+__global__ void __launch_bounds__(TH <= 32 ? 256 : TH, TH > 32 ? 512 / TH : NV * kPiece<T> > 32 ? 2 : 4)
     distill_fwd_kernel(const T *__restrict__ x, const float *__restrict__ values, const int64_t *__restrict__ indices, const float *__restrict__ rest,
                        const float *__restrict__ weight, float *__restrict__ row_loss, float *__restrict__ stats, float *__restrict__ listed, T *grad, DistillArgs a)
 {
@@ -233,8 +241,10 @@ __global__ void __launch_bounds__(TH <= 32 ? 256 : TH, TH <= 32 ? 2 : 512 / TH)
             }
             sums = make_float4(s.m, s.l, u.m, u.l);
         }
-        const RowNumbers num = row_numbers(mine, ExpSum{sums.x, sums.y}, ExpSum{sums.z, sums.w}, rs, w, a);
+        const TeacherNumbers teach = teacher_numbers(ExpSum{sums.z, sums.w}, rs, w, a);
+        const RowNumbers num = row_numbers(mine, ExpSum{sums.x, sums.y}, teach, a);
         const float m = num.m, coef = num.coef;
+        const bool there = teach.factor != 0.f && num.ul != 0.f;
         T *out = grad ? grad + r * a.classes : nullptr;
         if (grad) {
             const bool aligned = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(row.row)) & 15) == 0;
@@ -266,17 +276,19 @@ __global__ void __launch_bounds__(TH <= 32 ? 256 : TH, TH <= 32 ? 2 : 512 / TH)
         }
         // ---- the list again: its loss, and the gradient of its classes
         float loss = 0.f, own_grad = 0.f;
+        float log_tl = 0.f, log_ul = 0.f;
+        if (TH <= 32 || warp < list_warps) log_tl = logf(teach.tl), log_ul = logf(num.ul);
         auto gradient_of = [&](int n, const Entry &e) {
-            if (!num.there || e.cls < 0) return 0.f;
-            const float lp = num.log_p(e.t, tt), lq = num.log_q(e.s, tt), p = expf(lp);
+            if (!there || e.cls < 0) return 0.f;
+            const float lp = (e.t / tt - teach.tm) - log_tl, lq = (e.s - num.um) / tt - log_ul, p = expf(lp);
             if (p > 0.f || p != p) loss += p * (lp - lq);
             float mass = p;
             if ((twins >> (n / TH)) & 1) { // a class that is listed twice has both entries' probability
                 mass = 0.f;
                 for (int o = 0; o < a.k; ++o)
-                    if (list[o] == e.cls) mass += expf(num.log_p(val[o], tt));
+                    if (list[o] == e.cls) mass += expf((val[o] / tt - teach.tm) - log_tl);
             }
-            return num.factor * (expf(lq) - mass);
+            return teach.factor * (expf(lq) - mass);
         };
         if (TH > 32) {
             if (warp < list_warps) {
@@ -299,70 +311,170 @@ __global__ void __launch_bounds__(TH <= 32 ? 256 : TH, TH <= 32 ? 2 : 512 / TH)
                 loss = 0.f;
                 for (int i = 0; i < list_warps; ++i) loss += loss_part[i];
             }
-            row_loss[r] = num.loss(loss, rs, tt);
+            row_loss[r] = there ? num.loss(loss, teach, rs, tt) : 0.f;
             stats[2 * r] = m, stats[2 * r + 1] = coef;
         }
         team_sync(); // the tables are used again
     }
 }
 
-// Rows that are longer than a block's registers, many of them: a block reads its row twice, the second time for the gradient and from the L2, backwards.  What
-// is in flight (two rows an SM, or one of more than 256 KB) has to fit there.
-// The bit of a listed class is in a table of the whole row; a thread's 64 or 32 values of a trip have a word of it.
+constexpr int kTripPieces = 8; // of a thread
+
+// Rows that are longer than a block's registers, many of them: a block a row, twice, the second time for the gradient, backwards and from the L2 (which is why
+// no more rows are in flight than fit there).  The last warp does what a row's list asks for while the others read or write: its sums before the barrier
+// between the passes; loss, gradients and the next row's bits before the one behind them.  The bit of a listed class is in a table of the whole row, one for
+// rows of even and one for rows of odd number; a thread's values of a trip have 32 neighbouring bits, or two words.
 template <typename T, int TH>
 __global__ void __launch_bounds__(TH, 1024 / TH)
     distill_stream_kernel(const T *__restrict__ x, const float *__restrict__ values, const int64_t *__restrict__ indices, const float *__restrict__ rest,
                           const float *__restrict__ weight, float *__restrict__ row_loss, float *__restrict__ stats, float *__restrict__ listed, T *grad,
                           DistillArgs a)
 {
-    constexpr int NV = 8, EV = kPiece<T>, WARPS = TH / 32, WORDS = NV * EV / 32;
-    extern __shared__ uint32_t struck[]; // [trips][WORDS][TH]
+    constexpr int MT = TH - 32, NV = kTripPieces, EV = kPiece<T>, WORDS = NV * EV / 32, EACH = CLB_TOP_MAX / 32;
+    extern __shared__ uint32_t tables[]; // [2][trips][WORDS][MT]
+    const int words = a.chunks * WORDS * MT;
+    __shared__ ExpSum part[32];
+    __shared__ float4 from_list; // maximum and sum of the distinct listed scores, the teacher's probability of the rest, the gradient's factor
     __shared__ int list[CLB_TOP_MAX];
-    __shared__ ExpSum part[WARPS];
-    __shared__ float4 list_part[4];
-    __shared__ float loss_part[4];
-    const int t = threadIdx.x, lane = t & 31, warp = t >> 5, list_warps = (a.k + 31) / 32;
+    const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const float tt = a.temperature;
-    for (int i = t; i < a.chunks * WORDS * TH; i += TH) struck[i] = 0;
-    // a row's list and numbers are asked for while the row before it is written
-    long long next_cls = -1;
-    float next_t = -INFINITY, next_w = 1.f, next_rest = -INFINITY;
-    auto ask = [&](long long r) {
-        if (r >= a.rows) return;
-        if (t < a.k) next_cls = indices[r * a.k + t], next_t = values[r * a.k + t];
-        if (weight) next_w = weight[r];
-        if (rest) next_rest = rest[r];
-    };
-    ask(blockIdx.x);
+    for (int i = t; i < 2 * words; i += TH) tables[i] = 0;
+    if (t < 32) part[t] = ExpSum{-INFINITY, 0.f};
     __syncthreads();
-    for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
-        const RowPieces<T> row(x + r * a.stride, a.classes);
-        const float w = next_w, rs = next_rest;
-        Entry own{-1, -INFINITY, -INFINITY};
-        int word = 0;
-        bool twice = false;
-        if (t < a.k && next_cls >= 0 && next_cls < a.classes) {
-            own.cls = (int)next_cls, own.t = next_t, own.s = to_f(row.row[own.cls]);
-            const int j = row.piece_of(own.cls), bit = j / TH % NV * EV + row.place_of(own.cls);
-            word = (j / (TH * NV) * WORDS + (bit >> 5)) * TH + j % TH;
-            twice = (atomicOr(&struck[word], 1u << (bit & 31)) >> (bit & 31)) & 1;
+    if (warp == MT / 32) { // ---------------- the list
+        // Two rows ahead: classes and values are asked for; one ahead: their scores, and they are marked.  Each has a row's time to arrive.
+        struct {
+            int cls[EACH];
+            float t[EACH], s[EACH], w, rest;
+        } now, next;
+        long long ahead_cls[EACH];
+        float ahead_t[EACH], ahead_w = 1.f, ahead_rest = -INFINITY, g[EACH];
+        auto ask = [&](long long r) {
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const int n = lane + 32 * i;
+                const bool there = r < a.rows && n < a.k;
+                ahead_cls[i] = there ? indices[r * a.k + n] : -1;
+                ahead_t[i] = there ? values[r * a.k + n] : -INFINITY;
+            }
+            if (r < a.rows && weight) ahead_w = weight[r];
+            if (r < a.rows && rest) ahead_rest = rest[r];
+        };
+        auto take = [&](long long r) { // what was asked for becomes the next row
+            next.w = ahead_w, next.rest = ahead_rest;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                const bool there = ahead_cls[i] >= 0 && ahead_cls[i] < a.classes;
+                next.cls[i] = there ? (int)ahead_cls[i] : -1, next.t[i] = there ? ahead_t[i] : -INFINITY;
+                next.s[i] = there ? to_f(x[r * a.stride + next.cls[i]]) : -INFINITY;
+            }
+        };
+        auto place = [&](const T *row, int c) { // bit of a class in a table
+            const int v = c + (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T)), j = v / EV;
+            const int bit = j / MT % NV * EV + v % EV;
+            return (((j / (MT * NV)) * WORDS + (bit >> 5)) * MT + j % MT) * 32 + (bit & 31);
+        };
+        auto mark = [&](long long r, uint32_t *table) { // the next row's classes; is one listed twice?
+            bool twice = false;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i)
+                if (next.cls[i] >= 0) {
+                    const int at = place(x + r * a.stride, next.cls[i]);
+                    twice = twice || ((atomicOr(&table[at >> 5], 1u << (at & 31)) >> (at & 31)) & 1);
+                }
+            return (bool)__any_sync(0xffffffffu, twice);
+        };
+        ask(blockIdx.x);
+        take(blockIdx.x);
+        ask((long long)blockIdx.x + gridDim.x);
+        bool dup = false, next_dup = mark(blockIdx.x, tables);
+        int odd = 0;
+        __syncthreads();
+        for (long long r = blockIdx.x; r < a.rows; r += gridDim.x, odd ^= 1) {
+            const T *row = x + r * a.stride;
+            now = next, dup = next_dup;
+            int(&cls)[EACH] = now.cls;
+            float(&tv)[EACH] = now.t;
+            float(&sv)[EACH] = now.s;
+            const float w = now.w, rs = now.rest;
+            take(r + gridDim.x);
+            ask(r + 2 * (long long)gridDim.x);
+            if (dup) { // (rare)
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < EACH; ++i) list[lane + 32 * i] = cls[i];
+                __syncwarp();
+            }
+            ExpSum sk{-INFINITY, 0.f}, tk{-INFINITY, 0.f};
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) sk.m = fmaxf(sk.m, sv[i]), tk.m = fmaxf(tk.m, tv[i]);
+            sk.m = lanes_max<32>(sk.m), tk.m = lanes_max<32>(tk.m);
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                if (cls[i] < 0) continue;
+                bool first = true;
+                if (dup)
+                    for (int o = 0; o < lane + 32 * i; ++o) first = first && list[o] != cls[i];
+                if (first) sk.l += exp_of(sv[i], finite_or_zero(sk.m), a.c);
+                tk.l += exp_of(tv[i], finite_or_zero(tk.m), a.c);
+            }
+            sk.l = lanes_sum<32>(sk.l), tk.l = lanes_sum<32>(tk.l);
+            const TeacherNumbers q = teacher_numbers(tk, rs, w, a);
+            if (lane == 0) from_list = make_float4(sk.m, sk.l, q.rest, q.factor);
+            __syncthreads(); // ------------ all sums are there
+            const RowNumbers n = row_numbers(lanes_merge<32>(part[lane], a.c), sk, q, a);
+            const bool there = q.factor != 0.f && n.ul != 0.f;
+            const float log_tl = logf(q.tl), log_ul = logf(n.ul);
+            float loss = 0.f;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i) {
+                g[i] = 0.f;
+                if (there && cls[i] >= 0) {
+                    const float lp = (tv[i] / tt - q.tm) - log_tl, lq = (sv[i] - n.um) / tt - log_ul, p = expf(lp);
+                    if (p > 0.f || p != p) loss += p * (lp - lq);
+                    float mass = p;
+                    if (dup) { // a class that is listed twice has both entries' probability
+                        mass = 0.f;
+                        for (int o = 0; o < a.k; ++o)
+                            if (list[o] == cls[i]) mass += expf((values[r * a.k + o] / tt - q.tm) - log_tl);
+                    }
+                    g[i] = q.factor * (expf(lq) - mass);
+                }
+                if (lane + 32 * i < a.k) listed[r * a.k + lane + 32 * i] = g[i];
+            }
+            loss = lanes_sum<32>(loss);
+            if (lane == 0) {
+                row_loss[r] = there ? n.loss(loss, q, rs, tt) : 0.f;
+                stats[2 * r] = n.m, stats[2 * r + 1] = n.coef;
+            }
+            next_dup = mark(r + gridDim.x, tables + (odd ^ 1) * words);
+            __syncthreads(); // ------------ the row is written, the next one is marked
+            T *out = grad ? grad + r * a.classes : nullptr;
+#pragma unroll
+            for (int i = 0; i < EACH; ++i)
+                if (cls[i] >= 0) {
+                    if (grad) out[cls[i]] = from_f<T>(g[i]);
+                    const int at = place(row, cls[i]);
+                    atomicAnd(&tables[odd * words + (at >> 5)], ~(1u << (at & 31)));
+                }
         }
-        if (t < a.k) list[t] = own.cls;
-        const bool dup = __syncthreads_or(twice);
-        uint4 raw[NV];
+        return;
+    }
+    // -------------------------------------------- the row
+    int odd = 0;
+    uint4 raw[NV];
+    if (blockIdx.x < a.rows) RowPieces<T>(x + blockIdx.x * a.stride, a.classes).template load<NV, false>(raw, t, MT);
+    __syncthreads();
+    for (long long r = blockIdx.x; r < a.rows; r += gridDim.x, odd ^= 1) {
+        const RowPieces<T> row(x + r * a.stride, a.classes);
+        const uint32_t *const table = tables + odd * words;
         auto strike = [&](int trip) {
 #pragma unroll
-            for (int h = 0; h < WORDS; ++h)
-                if (const uint32_t m = struck[(trip * WORDS + h) * TH + t])
-#pragma unroll
-                    for (int i = 0; i < NV / WORDS; ++i)
-#pragma unroll
-                        for (int e = 0; e < EV; ++e)
-                            if ((m >> (i * EV + e)) & 1) drop_value<T>(raw[h * (NV / WORDS) + i], e);
+            for (int h = 0; h < WORDS; ++h) strike_out<T>(raw + h * (NV / WORDS), table[(trip * WORDS + h) * MT + t], NV / WORDS);
         };
         ExpSum mine{-INFINITY, 0.f};
         for (int trip = 0; trip < a.chunks; ++trip) {
-            row.template load<NV, false>(raw, trip * TH * NV + t, TH);
+            if (trip > 0) row.template load<NV, false>(raw, trip * MT * NV + t, MT);
             strike(trip);
             uint32_t top = low_word<T>();
 #pragma unroll
@@ -370,11 +482,14 @@ __global__ void __launch_bounds__(TH, 1024 / TH)
             const float m = fmaxf(mine.m, word_max<T>(top)), ref = finite_or_zero(m);
             const float before = mine.l * exp_of(mine.m, ref, a.c);
             const ExpRef er = exp_ref(ref, a.c);
-            float l[2] = {0.f, 0.f};
+            float sum = 0.f;
             if (!er.far) {
+                Pair l[2] = {pair_of(0.f, 0.f), pair_of(0.f, 0.f)};
 #pragma unroll
-                for (int i = 0; i < NV; ++i) piece_exp_sum<T>(l, raw[i], er.R, a.c);
-                l[0] = (l[0] + l[1]) * er.fix;
+                for (int i = 0; i < NV; ++i) piece_exp_sum<T>(l, raw[i], pair_of(-er.R, -er.R), pair_of(a.c, a.c));
+                float even, rest_of;
+                split(l[0] + l[1], even, rest_of);
+                sum = (even + rest_of) * er.fix;
             } else {
 #pragma unroll 1
                 for (int i = 0; i < NV; ++i) {
@@ -388,99 +503,58 @@ __global__ void __launch_bounds__(TH, 1024 / TH)
                         float f[Word<T>::n];
                         Word<T>::get(o[q], f);
 #pragma unroll
-                        for (int z = 0; z < Word<T>::n; ++z) l[0] += exp_of(f[z], ref, a.c);
+                        for (int z = 0; z < Word<T>::n; ++z) sum += exp_of(f[z], ref, a.c);
                     }
                 }
             }
-            mine = {m, before + l[0]};
+            mine = {m, before + sum};
         }
-        // ---- the list and the row
-        bool first = own.cls >= 0;
-        if (dup && first)
-            for (int o = 0; o < t; ++o) first = first && list[o] != own.cls;
         mine = lanes_merge<32>(mine, a.c);
         if (lane == 0) part[warp] = mine;
-        if (warp < list_warps) {
-            float4 sums;
-            sums.x = lanes_max<32>(own.s), sums.z = lanes_max<32>(own.t);
-            sums.y = lanes_sum<32>(first ? exp_of(own.s, finite_or_zero(sums.x), a.c) : 0.f);
-            sums.w = lanes_sum<32>(own.cls >= 0 ? exp_of(own.t, finite_or_zero(sums.z), a.c) : 0.f);
-            if (lane == 0) list_part[warp] = sums;
-        }
-        __syncthreads();
-        mine = lanes_merge<WARPS>(part[lane % WARPS], a.c);
-        ExpSum sk{list_part[0].x, list_part[0].y}, tk{list_part[0].z, list_part[0].w};
-        for (int i = 1; i < list_warps; ++i) {
-            sk = merge(sk, ExpSum{list_part[i].x, list_part[i].y}, a.c);
-            tk = merge(tk, ExpSum{list_part[i].z, list_part[i].w}, a.c);
-        }
-        const RowNumbers n = row_numbers(mine, sk, tk, rs, w, a);
-        float own_grad = 0.f;
-        if (warp < list_warps) {
-            float loss = 0.f;
-            if (n.there && own.cls >= 0) {
-                const float lp = n.log_p(own.t, tt), lq = n.log_q(own.s, tt), p = expf(lp);
-                if (p > 0.f || p != p) loss = p * (lp - lq);
-                float mass = p;
-                if (dup) { // a class that is listed twice has both entries' probability
-                    mass = 0.f;
-                    for (int o = 0; o < a.k; ++o)
-                        if (list[o] == own.cls) mass += expf(n.log_p(values[r * a.k + o], tt));
-                }
-                own_grad = n.factor * (expf(lq) - mass);
-            }
-            loss = lanes_sum<32>(loss);
-            if (lane == 0) loss_part[warp] = loss;
-            if (t < a.k) listed[r * a.k + t] = own_grad;
-        }
-        next_cls = -1;
-        ask(r + gridDim.x);
-        T *out = grad ? grad + r * a.classes : nullptr;
+        __syncthreads(); // ---------------- all sums are there
         if (grad) {
+            const float4 l = from_list;
+            TeacherNumbers q;
+            q.rest = l.z, q.factor = l.w;
+            const RowNumbers n = row_numbers(lanes_merge<32>(part[lane], a.c), ExpSum{l.x, l.y}, q, a);
+            T *out = grad + r * a.classes;
             const bool aligned = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(row.row)) & 15) == 0;
+            RowTrips<T, MT, NV> to(out, a.classes);
+            if (!aligned) to.hi = 0;
             const ExpRef er = exp_ref(n.m, a.c);
-            const float fixed = n.coef * er.fix;
+            const Pair c2 = pair_of(a.c, a.c), minus_R = pair_of(-er.R, -er.R), fixed = pair_of(n.coef * er.fix, n.coef * er.fix);
             for (int trip = a.chunks - 1; trip >= 0; --trip) {
-                const int base = trip * TH * NV + t;
                 if (trip < a.chunks - 1) {
-                    row.load(raw, base, TH);
+                    row.load(raw, trip * MT * NV + t, MT);
                     strike(trip);
                 }
-                auto gradients = [&](auto exponential) {
-                    const bool inside = aligned && row.template inside<NV>(base, TH);
+                auto gradients = [&](auto of_pair) {
 #pragma unroll
-                    for (int i = 0; i < NV; ++i) {
-                        uint32_t o[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    for (int q = 0; q < NV; ++q) {
+                        Pair v[kPairs<T>];
+                        piece_pairs<T>(raw[q], v);
 #pragma unroll
-                        for (int q = 0; q < 4; ++q) {
-                            float f[Word<T>::n];
-                            Word<T>::get(o[q], f);
-#pragma unroll
-                            for (int z = 0; z < Word<T>::n; ++z) f[z] = exponential(f[z]);
-                            o[q] = Word<T>::put(f);
-                        }
-                        const uint4 g = make_uint4(o[0], o[1], o[2], o[3]);
-                        if (inside) __stcs(reinterpret_cast<uint4 *>(out + row.first(base) + (long long)i * TH * EV), g);
-                        else if (base + i * TH < row.pieces) row.store(out, aligned, base + i * TH, g);
+                        for (int z = 0; z < kPairs<T>; ++z) v[z] = of_pair(v[z]);
+                        raw[q] = pairs_piece<T>(v);
                     }
                 };
-                if (n.coef == 0.f) gradients([](float) { return 0.f; }); // (a row that adds nothing may hold NaN)
-                else if (!er.far) gradients([&](float v) { return fixed * ex2(fmaf(v, a.c, -er.R)); });
-                else gradients([&](float v) { return n.coef * exp_of(v, n.m, a.c); });
+                if (n.coef == 0.f) gradients([](Pair) { return pair_of(0.f, 0.f); }); // (a row that adds nothing may hold NaN)
+                else if (!er.far) gradients([&](Pair v) { return fixed * ex2(fma2(v, c2, minus_R)); });
+                else gradients([&](Pair v) { return pair_of(n.coef, n.coef) * ex2((v + pair_of(-n.m, -n.m)) * c2); });
+                if (to.whole(trip)) {
+                    char *o = const_cast<char *>(to.at(trip));
+#pragma unroll
+                    for (int q = 0; q < NV; ++q) __stcs(reinterpret_cast<uint4 *>(o + q * MT * 16), raw[q]);
+                } else {
+                    const int base = trip * MT * NV + t;
+#pragma unroll
+                    for (int q = 0; q < NV; ++q)
+                        if (base + q * MT < row.pieces) row.store(out, aligned, base + q * MT, raw[q]);
+                }
             }
         }
-        __syncthreads(); // a listed class is written after the piece that it lies in
-        if (own.cls >= 0) {
-            if (grad) out[own.cls] = from_f<T>(own_grad);
-            struck[word] = 0;
-        }
-        if (t == 0) {
-            float loss = 0.f;
-            for (int i = 0; i < list_warps; ++i) loss += loss_part[i];
-            row_loss[r] = n.loss(loss, rs, tt);
-            stats[2 * r] = n.m, stats[2 * r + 1] = n.coef;
-        }
-        __syncthreads(); // the table is clear
+        if (r + gridDim.x < a.rows) RowPieces<T>(x + (r + gridDim.x) * a.stride, a.classes).template load<NV, false>(raw, t, MT);
+        __syncthreads(); // ---------------- the row is written, the next one is marked
     }
 }
 
@@ -590,9 +664,9 @@ template <typename T> long long most_pieces(const T *x, const DistillArgs &a)
 }
 template <typename T, int TH> cudaError_t launch_stream(const T *x, const FwdPointers &p, T *grad, DistillArgs a, long long pieces, cudaStream_t st)
 {
-    constexpr int NV = 8, WORDS = NV * kPiece<T> / 32;
-    a.chunks = (int)((pieces + TH * NV - 1) / (TH * NV));
-    const int bytes = a.chunks * WORDS * TH * 4;
+    constexpr int MT = TH - 32;
+    a.chunks = (int)((pieces + MT * kTripPieces - 1) / (MT * kTripPieces));
+    const int bytes = 2 * a.chunks * MT * kTripPieces * kPiece<T> / 8;
     const cudaError_t rc = ensure_dynamic_smem(distill_stream_kernel<T, TH>, bytes);
     if (rc != cudaSuccess) return rc;
     const long long most = (long long)sm_count() * (1024 / TH);
@@ -606,11 +680,22 @@ template <typename T> cudaError_t run_fwd(const T *x, const FwdPointers &p, T *g
     constexpr int NV = kValues / kPiece<T>;
     const long long pieces = most_pieces(x, a), block = 256 * NV;
     if (pieces <= 4) return launch_fwd<T, 4, 1, false>(x, p, grad, a, 0, pieces, st);
-    if (pieces <= 8 * NV) return launch_fwd<T, 8, NV, false>(x, p, grad, a, 0, pieces, st);
+    if (pieces <= 8 * NV / 4) return launch_fwd<T, 8, NV / 4, false>(x, p, grad, a, 0, pieces, st);
+    if (pieces <= 16 * NV / 2) return launch_fwd<T, 16, NV / 2, false>(x, p, grad, a, 0, pieces, st);
+    if (pieces <= 32 * NV / 2) return launch_fwd<T, 32, NV / 2, false>(x, p, grad, a, 0, pieces, st);
     if (pieces <= 32 * NV) return launch_fwd<T, 32, NV, false>(x, p, grad, a, 0, pieces, st);
-    if (pieces <= 128 * NV) return launch_fwd<T, 128, NV, false>(x, p, grad, a, 0, pieces, st);
-    if (pieces <= block) return launch_fwd<T, 256, NV, false>(x, p, grad, a, 0, pieces, st);
-    if (a.rows >= 64 && pieces <= 1200000 / kPiece<T>) return pieces <= 16384 ? launch_stream<T, 512>(x, p, grad, a, pieces, st) : launch_stream<T, 1024>(x, p, grad, a, pieces, st);
+    // A row of up to 16384 values in a block's registers where it fills most of them, else through the block twice.  134 million values with their gradient and
+    // lists of 64, registers / twice: 8192 of 8192 values fp32 260 / 285 us, bf16 206 / 251; 16384 of 16384 249 / 219, bf16 203 / 217; 4096 of 8192 418 / 382, bf16
+    // 371 / 246.  (A few rows are shared by clusters instead.)
+    const long long room = (pieces <= 128 * NV ? 128 : 256) * NV;
+    const bool many = a.rows >= 64 && a.classes <= 400000; // (two tables of 49 KB)
+    if (pieces <= block && (!many || 10 * pieces >= 7 * room))
+        return pieces <= 128 * NV ? launch_fwd<T, 128, NV, false>(x, p, grad, a, 0, pieces, st) : launch_fwd<T, 256, NV, false>(x, p, grad, a, 0, pieces, st);
+    if (many)
+        return pieces <= 768     ? launch_stream<T, 128>(x, p, grad, a, pieces, st)
+               : pieces <= 8192  ? launch_stream<T, 256>(x, p, grad, a, pieces, st)
+               : pieces <= 16384 ? launch_stream<T, 512>(x, p, grad, a, pieces, st)
+                                 : launch_stream<T, 1024>(x, p, grad, a, pieces, st);
     if (pieces <= 8 * block) return launch_fwd<T, 256, NV, true>(x, p, grad, a, pieces <= 2 * block ? 1 : pieces <= 4 * block ? 2 : 3, pieces, st);
     return launch_fwd<T, 512, NV, true>(x, p, grad, a, 3, pieces, st);
 }
