@@ -21,7 +21,6 @@ namespace {
 
 template <int NC> constexpr int kThreads = NC > 16 ? 128 : 256; // of a block (32 columns a lane: what four warps' sums take of shared memory)
 constexpr float kLog2e = 1.44269504f;
-constexpr uint32_t kMasked = 0x007fffffu; // order_key(-inf)
 
 // The columns of lane t of G: pieces of 16 bytes (VEC: rows at multiples of 16 bytes, whole pieces), or every G-th column.  Ascending either way.
 template <typename T, int G, int NC, bool VEC> __device__ __forceinline__ int column(int i, int t)
@@ -55,8 +54,8 @@ template <typename T, int G, int NC, bool VEC> __device__ __forceinline__ void l
         for (int i = 0; i < NC; ++i) v[i] = i * G + t < experts ? to_f(row[i * G + t]) : -INFINITY;
     }
 }
-// v becomes the row's probabilities; false for a row without a logit above -inf (NaN is one)
-template <int G, int NC> __device__ __forceinline__ bool soft_max(float (&v)[NC])
+// v becomes the row's probabilities; 0 for a row without a logit above -inf (whose v is then NaN), NaN for one that holds NaN
+template <int G, int NC> __device__ __forceinline__ float soft_max(float (&v)[NC])
 {
     float m = v[0];
 #pragma unroll
@@ -73,9 +72,11 @@ template <int G, int NC> __device__ __forceinline__ bool soft_max(float (&v)[NC]
     const float inv = 1.f / l;
 #pragma unroll
     for (int i = 0; i < NC; ++i) v[i] *= inv;
-    return l != 0.f;
+    return l;
 }
 
+// Choices are found among the logits themselves: the largest, the first of equal ones, then it becomes -inf, which is never chosen (NaN counts as +inf).
+// Their counts are bytes in a lane's registers, handed to the block every 255 rows.
 template <typename T, int G, int NC, bool VEC>
 __global__ void __launch_bounds__(kThreads<NC>) balance_fwd_kernel(const T *__restrict__ x, long long stride, const uint8_t *__restrict__ keep,
                                                                float *__restrict__ sums, int *__restrict__ counts, int *__restrict__ kept, int rows, int experts,
@@ -83,74 +84,87 @@ __global__ void __launch_bounds__(kThreads<NC>) balance_fwd_kernel(const T *__re
 {
     constexpr int TEAMS = kThreads<NC> / G, WARPS = kThreads<NC> / 32;
     __shared__ float psum[WARPS][G * NC];
-    __shared__ int cnt[WARPS][G * NC], all[WARPS];
+    __shared__ int cnt[G * NC], all[WARPS];
     const int t = threadIdx.x % G, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int e = threadIdx.x; e < G * NC; e += kThreads<NC>) cnt[e] = 0;
+    __syncthreads();
     float acc[NC];
-    int own[NC], mine = 0;
+    uint32_t own[NC / 4];
+    int mine = 0, since = 0;
 #pragma unroll
-    for (int i = 0; i < NC; ++i) acc[i] = 0.f, own[i] = 0;
+    for (int i = 0; i < NC; ++i) acc[i] = 0.f;
+#pragma unroll
+    for (int i = 0; i < NC / 4; ++i) own[i] = 0;
+    auto hand_over = [&] { // (whole numbers: any order)
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            int n = (own[i / 4] >> (i % 4 * 8)) & 0xff;
+            if (G == 1) n = __reduce_add_sync(0xffffffffu, n);
+            if (n && (G > 1 || lane == 0)) atomicAdd(&cnt[column<T, G, NC, VEC>(i, t)], n);
+        }
+#pragma unroll
+        for (int i = 0; i < NC / 4; ++i) own[i] = 0;
+        since = 0;
+    };
     // the teams of a warp take their turns together
     const int of_warp = blockIdx.x * TEAMS + (G < 32 ? warp * (32 / G) : warp);
     for (long long r0 = of_warp; r0 < rows; r0 += (long long)gridDim.x * TEAMS) {
         const long long r = r0 + lane / G;
         const bool live = r < rows && (!keep || keep[r]);
-        float v[NC];
+        float v[NC], u[NC];
 #pragma unroll
         for (int i = 0; i < NC; ++i) v[i] = -INFINITY;
         if (live) load_row<T, G, NC, VEC>(v, x + r * stride, t, experts);
-        uint32_t key[NC];
 #pragma unroll
-        for (int i = 0; i < NC; ++i) key[i] = order_key(v[i]);
-        if (!soft_max<G, NC>(v)) {
+        for (int i = 0; i < NC; ++i) u[i] = v[i];
+        const float l = soft_max<G, NC>(v);
+        if (l != 0.f) mine += t == 0; // (NaN is a row, too)
+        if (l != l)
 #pragma unroll
-            for (int i = 0; i < NC; ++i) v[i] = 0.f, key[i] = 0;
-        } else
-            mine += t == 0;
+            for (int i = 0; i < NC; ++i) u[i] = u[i] != u[i] ? INFINITY : u[i];
 #pragma unroll
-        for (int i = 0; i < NC; ++i) acc[i] += v[i];
+        for (int i = 0; i < NC; ++i) acc[i] += l != 0.f ? v[i] : 0.f;
         for (int n = 0; n < k; ++n) {
-            uint32_t best = key[0];
+            float best = u[0];
             int at = 0;
 #pragma unroll
             for (int i = 1; i < NC; ++i)
-                if (key[i] > best) best = key[i], at = i;
-            uint32_t top = best;
-            int col = column<T, G, NC, VEC>(at, t);
+                if (u[i] > best) best = u[i], at = i;
+            float top = best;
             if (G > 1) {
-#pragma unroll
-                for (int o = G / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+                top = lanes_max<G>(best);
+                const int col = column<T, G, NC, VEC>(at, t);
                 int first = best == top ? col : 0x7fffffff;
 #pragma unroll
                 for (int o = G / 2; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-                if (first != col || best != top) at = -1;
+                if (first != col) at = -1;
             }
-            if (top <= kMasked) at = -1; // nothing is left to choose
+            if (top == -INFINITY) at = -1; // nothing is left to choose
 #pragma unroll
-            for (int i = 0; i < NC; ++i)
-                if (i == at) ++own[i], key[i] = 0;
+            for (int i = 0; i < NC / 4; ++i) own[i] += at >> 2 == i ? 1u << ((at & 3) * 8) : 0u;
+            if (n + 1 < k)
+#pragma unroll
+                for (int i = 0; i < NC; ++i) u[i] = i == at ? -INFINITY : u[i];
         }
+        if (++since == 255) hand_over();
     }
-    // the teams of a warp, then the warps, each in order
+    hand_over();
+    // probabilities: the teams of a warp, then the warps, each in order
 #pragma unroll
     for (int i = 0; i < NC; ++i) {
 #pragma unroll
-        for (int o = 16; o >= G; o >>= 1) {
-            acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
-            own[i] += __shfl_xor_sync(0xffffffffu, own[i], o);
-        }
-        if (lane < G) psum[warp][column<T, G, NC, VEC>(i, t)] = acc[i], cnt[warp][column<T, G, NC, VEC>(i, t)] = own[i];
+        for (int o = 16; o >= G; o >>= 1) acc[i] += __shfl_xor_sync(0xffffffffu, acc[i], o);
+        if (lane < G) psum[warp][column<T, G, NC, VEC>(i, t)] = acc[i];
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
+    mine = __reduce_add_sync(0xffffffffu, mine);
     if (lane == 0) all[warp] = mine;
     __syncthreads();
     for (int e = threadIdx.x; e < experts; e += kThreads<NC>) {
         float p = 0.f;
-        int c = 0;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) p += psum[w][e], c += cnt[w][e];
+        for (int w = 0; w < WARPS; ++w) p += psum[w][e];
         sums[(long long)blockIdx.x * experts + e] = p;
-        counts[(long long)blockIdx.x * experts + e] = c;
+        counts[(long long)blockIdx.x * experts + e] = cnt[e];
     }
     if (threadIdx.x == 0) {
         int m = 0;
@@ -223,7 +237,7 @@ __global__ void __launch_bounds__(kThreads<NC>) balance_bwd_kernel(const T *__re
 #pragma unroll
         for (int i = 0; i < NC; ++i) v[i] = -INFINITY;
         if (kept) load_row<T, G, NC, VEC>(v, x + r * stride, t, experts);
-        const bool there = soft_max<G, NC>(v) && kept;
+        const bool there = soft_max<G, NC>(v) != 0.f && kept;
         float dot = 0.f;
 #pragma unroll
         for (int i = 0; i < NC; ++i) dot += v[i] * h[i];
@@ -273,10 +287,10 @@ int teams_of(int64_t experts) // of a block
     with_team(experts, [&](auto G, auto NC) { n = kThreads<decltype(NC)::value> / decltype(G)::value; });
     return n;
 }
-// Blocks of the forward pass: up to six an SM, and sums of at most 512 KB for the one block that finishes.
+// Blocks of the forward pass: up to four an SM, and sums of at most 512 KB for the one block that finishes.
 int balance_blocks(int64_t rows, int64_t experts)
 {
-    const int64_t teams = teams_of(experts), most = std::min<int64_t>(6 * 148, std::max<int64_t>(64, 65536 / experts));
+    const int64_t teams = teams_of(experts), most = std::min<int64_t>(4 * 148, std::max<int64_t>(64, 65536 / experts));
     return (int)std::min<int64_t>((rows + teams - 1) / teams, most);
 }
 template <typename T> bool whole_pieces(const void *x, int64_t stride, int64_t experts)
