@@ -182,6 +182,20 @@ __global__ void __launch_bounds__(kBlock, 4) top_select_kernel(const T *__restri
                     if (g[z] < reach) l += ex2(fmaf(g[z], a.c, -er.R));
             }
         }
+        if constexpr (TH == 32) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if ((hits >> i) & 1)
+#pragma unroll
+                    for (int e = 0; e < EV; ++e) {
+                        const float v = value_at(i, e);
+                        if (!(v < reach) || few) {
+                            const int cls = class_of(i, e);
+                            if (cls >= 0 && (!(v < reach) || cls < a.k)) push(v, cls);
+                        }
+                    }
+            hits = 0;
+        }
         while (hits) { // read once more: a warp has as many turns as its lanes have such pieces at most, one or two, not one for every piece
             const int i = __ffs(hits) - 1;
             hits &= hits - 1;
