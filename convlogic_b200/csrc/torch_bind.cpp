@@ -1026,6 +1026,11 @@ Rows rows_of(const Tensor &x, const char *what)
     TORCH_CHECK_VALUE(x.size(-1) > 0, "convlogic_b200: ", what, " have no classes");
     const int64_t classes = x.size(-1), rows = x.numel() / classes;
     Rows out{Tensor(), rows, classes, classes, score_dtype(x)};
+    if (x.dim() == 2 && x.stride(1) == 1) { // as it is
+        out.x = x;
+        out.stride = rows > 1 ? x.stride(0) : classes;
+        return out;
+    }
     // (a row of one class, or a tensor of one row, may have any stride there)
     out.x = classes == 1 || x.stride(-1) == 1 ? x.reshape({rows, classes}) : x.contiguous().view({rows, classes});
     if (classes > 1 && out.x.stride(1) != 1) out.x = out.x.contiguous();
@@ -1082,7 +1087,7 @@ Lists lists_of(const Tensor &scores, const Tensor &values, const Tensor &indices
     auto prepared = [&](const Tensor &t, const char *what, at::ScalarType type) {
         TORCH_CHECK(t.device() == scores.device(), "convlogic_b200: ", what, " must be on ", scores.device(), ", got ", t.device());
         TORCH_CHECK(!(at::GradMode::is_enabled() && t.requires_grad()), "convlogic_b200: ", what, " gets no gradient: detach it");
-        return t.detach().to(type).contiguous();
+        return t.scalar_type() == type && t.is_contiguous() ? t : t.detach().to(type).contiguous();
     };
     out.values = prepared(values, "the lists' values", at::kFloat);
     out.indices = prepared(indices, "the lists' indices", at::kLong);
@@ -1096,31 +1101,33 @@ Lists lists_of(const Tensor &scores, const Tensor &values, const Tensor &indices
 }
 
 struct Distilled {
-    Tensor loss, stats, listed, grad;
+    Tensor loss, kept, grad; // kept: [rows][2] stats, [rows][k] listed, and behind them the call's scratch
+    float *stats = nullptr, *listed = nullptr;
 };
 Distilled distill_fwd(const Rows &x, const Tensor &like, const Lists &l, double temperature, int reduction, bool want_grad = false)
 {
     Below below(x.x);
     Distilled out;
     out.loss = reduction == CLB_REDUCE_NONE ? alloc(row_shape(like), x.x, at::kFloat) : alloc({}, x.x, at::kFloat);
-    out.stats = alloc({x.rows, 2}, x.x, at::kFloat), out.listed = alloc({x.rows, l.k}, x.x, at::kFloat);
+    const size_t bytes = clb_distill_scratch_bytes(x.rows, x.classes, (int)l.k);
+    const int64_t kept = x.rows * (l.k + 2);
+    out.kept = alloc({kept + (int64_t)(bytes + 3) / 4}, x.x, at::kFloat);
+    out.stats = ptr<float>(out.kept), out.listed = out.stats + 2 * x.rows;
     if (x.rows == 0 && reduction == CLB_REDUCE_NONE) return out;
     if (want_grad) out.grad = alloc(like.sizes(), x.x);
-    const size_t bytes = clb_distill_scratch_bytes(x.rows, x.classes, (int)l.k);
-    Tensor scratch = scratch_bytes(bytes, x.x);
     check(clb_distill_fwd(ptr(x.x), x.stride, ptr<float>(l.values), ptr<int64_t>(l.indices), ptr<float>(l.rest), ptr<float>(l.weight), ptr<float>(out.loss),
-                          ptr<float>(out.stats), ptr<float>(out.listed), ptr(out.grad), ptr(scratch), bytes, x.rows, x.classes, (int)l.k, temperature, reduction, x.dtype,
+                          out.stats, out.listed, ptr(out.grad), out.stats + kept, bytes, x.rows, x.classes, (int)l.k, temperature, reduction, x.dtype,
                           cur_stream()));
     return out;
 }
-Tensor distill_bwd(const Rows &x, at::IntArrayRef sizes, const Tensor &indices, const Tensor &stats, const Tensor &listed, const Tensor &up, bool per_row,
+Tensor distill_bwd(const Rows &x, at::IntArrayRef sizes, const Tensor &indices, const float *stats, const float *listed, int64_t k, const Tensor &up, bool per_row,
                    double temperature, Tensor unit = Tensor())
 {
     Below below(x.x);
     Tensor g = unit.defined() ? unit : alloc(sizes, x.x);
     if (x.rows)
-        check(clb_distill_bwd(ptr(x.x), x.stride, ptr<int64_t>(indices), ptr<float>(stats), ptr<float>(listed), ptr<float>(up), per_row, unit.defined(),
-                              ptr(g), x.rows, x.classes, (int)listed.size(1), temperature, x.dtype, cur_stream()));
+        check(clb_distill_bwd(ptr(x.x), x.stride, ptr<int64_t>(indices), stats, listed, ptr<float>(up), per_row, unit.defined(),
+                              ptr(g), x.rows, x.classes, (int)k, temperature, x.dtype, cur_stream()));
     return g;
 }
 
@@ -1134,6 +1141,8 @@ variable_list once(Tensor g, const Tensor &x)
     }
     return {g};
 }
+
+Tensor plain_float(const Tensor &t) { return t.scalar_type() == at::kFloat && t.is_contiguous() ? t : t.detach().to(at::kFloat).contiguous(); }
 
 // Which capture the current stream records into, 0 for none.
 unsigned long long capture_id()
@@ -1149,7 +1158,8 @@ unsigned long long capture_id()
 // capture as the forward (or, like it, in none): a graph of the backward alone has to write its result at every replay, and a graph of the forward
 // would write over a result handed out.  Not for fp16, whose losses are scaled, nor for losses of rows.
 struct DistillNode : public Node {
-    SavedVariable x, indices, stats, listed;
+    SavedVariable x, indices, kept;
+    int64_t k;
     Tensor unit; // of the first backward call
     unsigned long long capture = 0;
     int reduction;
@@ -1158,7 +1168,7 @@ struct DistillNode : public Node {
     void release_variables() override
     {
         std::lock_guard<std::mutex> lock(mutex_);
-        x.reset_data(), indices.reset_data(), stats.reset_data(), listed.reset_data(), unit.reset();
+        x.reset_data(), indices.reset_data(), kept.reset_data(), unit.reset();
     }
     Tensor take_unit()
     {
@@ -1169,12 +1179,14 @@ struct DistillNode : public Node {
     {
         const Tensor xx = x.unpack();
         c10::cuda::CUDAGuard device(xx.device());
-        const Tensor up = upstream(*this, grads).detach().to(at::kFloat).contiguous();
+        const Tensor up = plain_float(upstream(*this, grads));
         Tensor g;
         {
             at::NoGradGuard no_grad;
-            g = distill_bwd(rows_of(xx, "the scores"), xx.sizes(), indices.unpack(), stats.unpack(), listed.unpack(), up, reduction == CLB_REDUCE_NONE,
-                            temperature, take_unit());
+            const Rows rows = rows_of(xx, "the scores");
+            const Tensor state = kept.unpack();
+            g = distill_bwd(rows, xx.sizes(), indices.unpack(), ptr<float>(state), ptr<float>(state) + 2 * rows.rows, k, up, reduction == CLB_REDUCE_NONE, temperature,
+                            take_unit());
         }
         return once(g, xx);
     }
@@ -1206,7 +1218,7 @@ Tensor distillation_loss(const Tensor &x_in, const Tensor &values, const Tensor 
     if (grad) {
         auto node = new_node<DistillNode>();
         node->set_next_edges(torch::autograd::collect_next_edges(x_in));
-        node->x = saved(x_in), node->indices = saved(l.indices), node->stats = saved(out.stats), node->listed = saved(out.listed);
+        node->x = saved(x_in), node->indices = saved(l.indices), node->kept = saved(out.kept), node->k = l.k;
         node->unit = out.grad, node->reduction = how, node->temperature = temperature;
         if (out.grad.defined()) {
             c10::cuda::CUDAGuard device(x_in.device());
@@ -1225,8 +1237,9 @@ std::tuple<Tensor, Tensor, Tensor> distill_fwd_py(const Tensor &x_in, const Tens
     const int how = reduction_code(reduction);
     check_temperature(temperature);
     const Rows x = rows_of(x_in, "the scores");
-    Distilled out = distill_fwd(x, x_in, lists_of(x_in, values, indices, rest, weight), temperature, how);
-    return {out.loss, out.stats, out.listed};
+    const Lists l = lists_of(x_in, values, indices, rest, weight);
+    Distilled out = distill_fwd(x, x_in, l, temperature, how);
+    return {out.loss, out.kept.narrow(0, 0, 2 * x.rows).view({x.rows, 2}), out.kept.narrow(0, 2 * x.rows, x.rows * l.k).view({x.rows, l.k})};
 }
 Tensor distill_bwd_py(const Tensor &up, const Tensor &x_in, const Tensor &indices, const Tensor &stats, const Tensor &listed, double temperature)
 {
@@ -1240,7 +1253,7 @@ Tensor distill_bwd_py(const Tensor &up, const Tensor &x_in, const Tensor &indice
                 "convlogic_b200: distill_bwd expects what distill_fwd returned for these scores");
     TORCH_CHECK(up.scalar_type() == at::kFloat && (up.dim() == 0 || up.numel() == x.rows),
                 "convlogic_b200: the upstream gradient must be one float32 value, or one for each row");
-    return distill_bwd(x, x_in.sizes(), indices, stats, listed, up, up.dim() != 0, temperature);
+    return distill_bwd(x, x_in.sizes(), indices, ptr<float>(stats), ptr<float>(listed), listed.size(1), up, up.dim() != 0, temperature);
 }
 
 // ---- balance over experts
@@ -1286,7 +1299,7 @@ struct BalanceNode : public Node {
     {
         const Tensor xx = x.unpack();
         c10::cuda::CUDAGuard device(xx.device());
-        const Tensor up = upstream(*this, grads).detach().to(at::kFloat).contiguous();
+        const Tensor up = plain_float(upstream(*this, grads));
         Tensor g;
         {
             at::NoGradGuard no_grad;
