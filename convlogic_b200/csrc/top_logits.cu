@@ -2,7 +2,7 @@
 //
 // A row's classes are ordered by value, ties by index; the first k are the list, and rest = log sum over the others of exp(x / T).
 //
-// One read of the logits.  A team of threads (a warp for rows of up to 1024 values; a block for a segment of 8192 fp32 or 16384 half values of a longer row, so
+// One read of the logits.  A team of threads (a warp for rows of up to 1024 fp32 or 2048 half values; a block for longer ones, or for a segment of 32 KB, so
 // that one row, too, fills part of the GPU) holds its values in registers:
 //   1. The k-th largest of the threads' own maxima, rounded down to 16 bits of its order, is a bound that at least k values reach, and few more: with 256 maxima
 //      of 64 values about 75 for k = 64.  One warp finds it by bisection.
@@ -98,13 +98,13 @@ template <int TH, typename F> __device__ __forceinline__ void ranked(const u64 *
     }
 }
 
-// TH threads a row (32) or a segment of one (256), NV pieces a thread.
-template <typename T, int TH, int NV>
-__global__ void __launch_bounds__(kBlock, 4) top_select_kernel(const T *__restrict__ x, float *__restrict__ values, int64_t *__restrict__ indices,
+// TH threads a row (32: teams of a block of 256; 64 to 256: a block) or a segment of one (256), NV pieces a thread.  TH * SUB groups.
+template <typename T, int TH, int NV, int SUB>
+__global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBlock / TH) top_select_kernel(const T *__restrict__ x, float *__restrict__ values, int64_t *__restrict__ indices,
                                                                float *__restrict__ rest, u64 *__restrict__ places, ExpSum *__restrict__ sums, TopArgs a)
 {
-    constexpr int TEAMS = kBlock / TH, EV = kPiece<T>, SUB = TH == 32 ? 4 : 1, CAP = TH == 32 ? 256 : 512;
-    static_assert(NV % SUB == 0, "groups of whole pieces");
+    constexpr int TEAMS = TH == 32 ? kBlock / TH : 1, EV = kPiece<T>, CAP = TH == 32 ? 256 : 512;
+    static_assert(NV % SUB == 0 || 2 * NV == SUB, "groups of whole or half pieces");
     __shared__ __align__(16) u64 cand_all[TEAMS][CAP + 2];
     __shared__ uint32_t keys_all[TEAMS][TH * SUB], extra_all[TEAMS][CAP];
     __shared__ int count_all[TEAMS], box[TH / 32 + 1];
@@ -137,9 +137,13 @@ __global__ void __launch_bounds__(kBlock, 4) top_select_kernel(const T *__restri
         for (int i = 0; i < NV; ++i) tops[i] = piece_max_nan<T>(raw[i]);
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
-            uint32_t top = tops[s * (NV / SUB)];
+            uint32_t top;
+            if constexpr (NV >= SUB) {
+                top = tops[s * (NV / SUB)];
 #pragma unroll
-            for (int i = 1; i < NV / SUB; ++i) top = max_nan<T>(top, tops[s * (NV / SUB) + i]);
+                for (int i = 1; i < NV / SUB; ++i) top = max_nan<T>(top, tops[s * (NV / SUB) + i]);
+            } else
+                top = s & 1 ? max_nan<T>(raw[s / 2].z, raw[s / 2].w) : max_nan<T>(raw[s / 2].x, raw[s / 2].y);
             keys_all[team][s * TH + t] = word_key<T>(top);
         }
         if (t == 0) count_all[team] = 0;
@@ -430,8 +434,7 @@ __global__ void __launch_bounds__(kBlock) top_merge_kernel(const u64 *__restrict
     }
 }
 
-constexpr int kWarpPieces(int size) { return size == 4 ? 8 : 4; } // 32 values a lane
-constexpr int kSegmentPieces = 8;                                 // 32 KB a block
+constexpr int kPieces = 8; // of a thread: 32 KB a block of 256
 
 // pieces of the longest row (rows at a multiple of 16 bytes all begin at the first one's place in its piece; with `any`, at the worst)
 template <typename T> long long most_pieces(const void *x, int64_t stride, int64_t rows, int64_t classes, bool any = false)
@@ -441,7 +444,7 @@ template <typename T> long long most_pieces(const void *x, int64_t stride, int64
 }
 template <typename T> int segments_of(long long pieces)
 {
-    return pieces <= 32 * kWarpPieces(sizeof(T)) ? 1 : (int)((pieces + kBlock * kSegmentPieces - 1) / (kBlock * kSegmentPieces));
+    return (int)((pieces + kBlock * kPieces - 1) / (kBlock * kPieces));
 }
 
 } // namespace
@@ -483,13 +486,18 @@ extern "C" int clb_top_logits(const void *x, int64_t row_stride, float *values, 
             else go(top_few_kernel<T, 4>);
             return;
         }
-        if (pieces <= 32 * kWarpPieces(sizeof(T))) {
-            CLB_TRACED("top_select_kernel", st,
-                       top_select_kernel<T, 32, kWarpPieces(sizeof(T))><<<blocks((rows + 7) / 8), kBlock, 0, st>>>((const T *)x, values, indices, rest, places, sums, a));
-            return;
-        }
-        CLB_TRACED("top_select_kernel", st,
-                   top_select_kernel<T, kBlock, kSegmentPieces><<<blocks(rows * a.segments), kBlock, 0, st>>>((const T *)x, values, indices, rest, places, sums, a));
+        auto go = [&](auto kernel, long long n, int threads) {
+            CLB_TRACED("top_select_kernel", st, kernel<<<blocks(n), threads, 0, st>>>((const T *)x, values, indices, rest, places, sums, a));
+        };
+        // Groups: more of them make a tighter bound and a longer search for it.  65536 rows of 1000 classes, 128 and 256 groups: k = 20 133 and 152 us, k = 100
+        // 582 and 362.
+        auto warps = [&](auto few, auto many) { go(k <= 32 ? few : many, (rows + 7) / 8, kBlock); };
+        constexpr int SHORT = sizeof(T) == 2 ? 4 : kPieces; // half types: 1024 values of a warp, or 2048
+        if (pieces <= 32 * SHORT) warps(top_select_kernel<T, 32, SHORT, 4>, top_select_kernel<T, 32, SHORT, 8>);
+        else if (pieces <= 32 * kPieces) warps(top_select_kernel<T, 32, kPieces, 4>, top_select_kernel<T, 32, kPieces, 8>);
+        else if (pieces <= 64 * kPieces) go(top_select_kernel<T, 64, kPieces, 4>, rows, 64);
+        else if (pieces <= 128 * kPieces) go(top_select_kernel<T, 128, kPieces, 2>, rows, 128);
+        else go(top_select_kernel<T, kBlock, kPieces, 1>, rows * a.segments, kBlock);
         if (a.segments > 1) {
             CLB_TRACED("top_merge_kernel", st, top_merge_kernel<<<blocks(rows), kBlock, 0, st>>>(places, sums, values, indices, rest, a));
             launches = 2;
