@@ -132,9 +132,11 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
             return f[Word<T>::n == 1 ? 0 : e & 1];
         };
         // ---- 1: the bound
+        // a warp's pieces from i * TH on are not there if that is not below `used` (blocks' rows fill most of theirs)
+        const int used = TH == 32 ? row.pieces - base : NV * TH;
         uint32_t tops[NV];
 #pragma unroll
-        for (int i = 0; i < NV; ++i) tops[i] = piece_max_nan<T>(raw[i]);
+        for (int i = 0; i < NV; ++i) tops[i] = i * TH < used ? piece_max_nan<T>(raw[i]) : low_word<T>();
 #pragma unroll
         for (int s = 0; s < SUB; ++s) {
             uint32_t top;
@@ -172,6 +174,7 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
         uint32_t hits = 0; // pieces with a candidate
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
+            if (i * TH >= used) continue;
             float f[Word<T>::n];
             Word<T>::get(tops[i], f);
             const bool hit = !(f[0] < reach) || !(f[Word<T>::n - 1] < reach) || (few && row.first(base + i * TH + t) < own_first + a.k);
