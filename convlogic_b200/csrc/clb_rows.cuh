@@ -290,7 +290,7 @@ template <int LANES> __device__ __forceinline__ float lanes_max(float v) // NaN 
 {
     if (LANES == 32) { // one instruction for the warp
         float r;
-        asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+        asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
         return r;
     }
 #pragma unroll

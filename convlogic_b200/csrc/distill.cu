@@ -605,19 +605,30 @@ __global__ void __launch_bounds__(256) distill_bwd_kernel(const T *__restrict__ 
     }
 }
 
-__global__ void __launch_bounds__(1024) distill_sum_kernel(const float *__restrict__ row_loss, float *__restrict__ loss, long long rows)
+// Sums of `n` numbers in a fixed order: block b those of its part, in 64 bits.  One block up to 2^18 rows (65536: 3 us), else 128 and then one over theirs.
+constexpr int kSumParts = 128;
+constexpr long long kOneSum = 1 << 18;
+template <typename In, typename Out> __global__ void __launch_bounds__(1024) distill_sum_kernel(const In *__restrict__ in, Out *__restrict__ out, long long n)
 {
-    __shared__ double red[1024];
+    __shared__ double red[32];
+    const long long lo = n * blockIdx.x / gridDim.x, hi = n * (blockIdx.x + 1) / gridDim.x;
     double mine = 0.0;
-    for (long long r = threadIdx.x; r < rows; r += 1024) mine += row_loss[r];
-    red[threadIdx.x] = mine;
-    __syncthreads();
-    for (int half = 512; half >= 1; half >>= 1) {
-        if ((int)threadIdx.x < half) red[threadIdx.x] += red[threadIdx.x + half];
-        __syncthreads();
+    for (long long r = lo + threadIdx.x; r < hi; r += 16 * 1024) {
+        In v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = r + i * 1024 < hi ? in[r + i * 1024] : In(0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) mine += v[i];
     }
-    if (threadIdx.x == 0) *loss = (float)red[0];
+    mine = warp_sum<double>(mine);
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = mine;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        mine = warp_sum<double>(red[threadIdx.x]);
+        if (threadIdx.x == 0) out[blockIdx.x] = (Out)mine;
+    }
 }
+size_t sums_at(int64_t rows) { return (size_t)((rows * 4 + 7) & ~7ll); } // of the parts' sums, behind the rows' losses
 
 bool sizes_ok(int64_t rows, int64_t classes, int64_t row_stride, int k, double temperature, int dtype)
 {
@@ -715,7 +726,7 @@ void launch_bwd(const T *x, const int64_t *indices, const float *stats, const fl
 extern "C" size_t clb_distill_scratch_bytes(int64_t rows, int64_t classes, int k)
 {
     if (rows <= 0 || classes <= 0 || k <= 0) return 0;
-    return (size_t)rows * 4;
+    return sums_at(rows) + (rows > kOneSum ? kSumParts * 8 : 0);
 }
 
 extern "C" int clb_distill_fwd(const void *scores, int64_t row_stride, const float *values, const int64_t *indices, const float *rest, const float *weight,
@@ -738,8 +749,14 @@ extern "C" int clb_distill_fwd(const void *scores, int64_t row_stride, const flo
         if (rc != cudaSuccess) return check_launch(0);
     }
     if (reduction == CLB_REDUCE_NONE) return rows > 0 ? check_launch() : CLB_OK;
-    CLB_TRACED("distill_sum_kernel", st, distill_sum_kernel<<<1, 1024, 0, st>>>((const float *)scratch, loss, rows));
-    return check_launch(rows > 0 ? 2 : 1);
+    if (rows <= kOneSum) {
+        CLB_TRACED("distill_sum_kernel", st, distill_sum_kernel<float, float><<<1, 1024, 0, st>>>((const float *)scratch, loss, rows));
+        return check_launch(rows > 0 ? 2 : 1);
+    }
+    double *const parts = (double *)((char *)scratch + sums_at(rows));
+    CLB_TRACED("distill_sum_kernel", st, distill_sum_kernel<float, double><<<kSumParts, 1024, 0, st>>>((const float *)scratch, parts, rows));
+    CLB_TRACED("distill_sum_kernel", st, distill_sum_kernel<double, float><<<1, 1024, 0, st>>>(parts, loss, kSumParts));
+    return check_launch(3);
 }
 
 extern "C" int clb_distill_bwd(const void *scores, int64_t row_stride, const int64_t *indices, const float *stats, const float *listed, const float *upstream,

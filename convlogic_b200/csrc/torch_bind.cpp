@@ -1051,7 +1051,7 @@ void check_top(int64_t k, int64_t classes)
     TORCH_CHECK_VALUE(k <= CLB_TOP_MAX, "convlogic_b200: lists have at most ", CLB_TOP_MAX, " classes, got ", k);
 }
 
-std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor &x_in, int64_t k, double temperature)
+std::tuple<Tensor, Tensor, Tensor> top_logits_raw(const Tensor &x_in, int64_t k, double temperature)
 {
     check_temperature(temperature);
     at::NoGradGuard no_grad;
@@ -1065,6 +1065,11 @@ std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor &x_in, int64_t k, dou
         check(clb_top_logits(ptr(x.x), x.stride, ptr<float>(values), ptr<int64_t>(indices), ptr<float>(rest), ptr(scratch), bytes, x.rows, x.classes, (int)k, temperature, x.dtype,
                              cur_stream()));
     return {values, indices, rest};
+}
+std::tuple<Tensor, Tensor, Tensor> top_logits(const Tensor &x_in, int64_t k, double temperature)
+{
+    if (torch::jit::tracer::isTracing()) return in_python("followed_top_logits", x_in, k, temperature).cast<std::tuple<Tensor, Tensor, Tensor>>();
+    return top_logits_raw(x_in, k, temperature);
 }
 
 // A teacher's lists as the kernels read them.
@@ -1101,7 +1106,7 @@ Lists lists_of(const Tensor &scores, const Tensor &values, const Tensor &indices
 }
 
 struct Distilled {
-    Tensor loss, kept, grad; // kept: [rows][2] stats, [rows][k] listed, and behind them the call's scratch
+    Tensor loss, kept, grad; // kept: [rows][2] stats, [rows][k] listed, and behind them (8-byte aligned) the call's scratch
     float *stats = nullptr, *listed = nullptr;
 };
 Distilled distill_fwd(const Rows &x, const Tensor &like, const Lists &l, double temperature, int reduction, bool want_grad = false)
@@ -1110,7 +1115,7 @@ Distilled distill_fwd(const Rows &x, const Tensor &like, const Lists &l, double 
     Distilled out;
     out.loss = reduction == CLB_REDUCE_NONE ? alloc(row_shape(like), x.x, at::kFloat) : alloc({}, x.x, at::kFloat);
     const size_t bytes = clb_distill_scratch_bytes(x.rows, x.classes, (int)l.k);
-    const int64_t kept = x.rows * (l.k + 2);
+    const int64_t kept = (x.rows * (l.k + 2) + 1) & ~1ll;
     out.kept = alloc({kept + (int64_t)(bytes + 3) / 4}, x.x, at::kFloat);
     out.stats = ptr<float>(out.kept), out.listed = out.stats + 2 * x.rows;
     if (x.rows == 0 && reduction == CLB_REDUCE_NONE) return out;
@@ -1312,7 +1317,7 @@ struct BalanceNode : public Node {
 std::tuple<Tensor, Tensor> balance_loss(const Tensor &x_in, int64_t k, const std::optional<Tensor> &keep)
 {
     if (followed({x_in})) return in_python("followed_balance_loss", x_in, k, keep).cast<std::tuple<Tensor, Tensor>>();
-    if (g_sinks.load(std::memory_order_relaxed) > 0 && x_in.requires_grad()) {
+    if (g_sinks.load(std::memory_order_relaxed) > 0 && wants_grad({x_in})) {
         py::gil_scoped_acquire gil;
         TORCH_CHECK(!sink_of(x_in), "convlogic_b200: these logits' gradient is written straight into a bucket by their layer (GradBucket.direct), "
                                     "which would overwrite the balance loss's: turn it off with direct(False)");
@@ -1555,6 +1560,7 @@ PYBIND11_MODULE(_clb_torch, m)
     m.def("group_sum_ce", &group_sum_ce);
     m.def("trees", &trees);
     m.def("top_logits", &top_logits);
+    m.def("top_logits_raw", &top_logits_raw);
     m.def("distillation_loss", &distillation_loss);
     m.def("distill_fwd", &distill_fwd_py);
     m.def("distill_bwd", &distill_bwd_py);

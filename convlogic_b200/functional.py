@@ -275,6 +275,20 @@ class LogicTreeCrossEntropyFunction(Function):
         return (gx, g0, g1, g2) + (None,) * 8
 
 
+class TopLogitsFunction(Function):
+    """The largest logits of every row and the mass of the others (``ops.top_logits``); no gradient."""
+
+    @staticmethod
+    def forward(ctx, x, k, temperature):
+        out = ops.top_logits(x, k, temperature)
+        ctx.mark_non_differentiable(*out)
+        return out
+
+    @staticmethod
+    def backward(ctx, *unused):
+        return None, None, None
+
+
 class DistillationFunction(Function):
     """Loss of scores against a teacher's lists of top logits (``ops.distill_fwd``); the lists and the weight get no gradient."""
 
@@ -352,6 +366,10 @@ def followed_trees(x, w0, w1, w2, leaf, node, start, slots, wmode, covers_all, l
     if labels is None:
         return LogicTreeFunction.apply(x_fm, w0, w1, w2, leaf, node, start, slots, wmode, covers_all).transpose(0, 1)
     return LogicTreeCrossEntropyFunction.apply(x_fm, w0, w1, w2, leaf, node, start, slots, labels, k, tau, covers_all)
+
+
+def followed_top_logits(*args):
+    return TopLogitsFunction.apply(*args)
 
 
 def followed_distillation_loss(*args):

@@ -502,7 +502,7 @@ def adam_step(p, g, m, v, lr, beta1, beta2, eps, weight_decay, step, decoupled):
 # ------------------------------------------------------------------------------------------- loss terms on rows of scores
 def top_logits(x, k, temperature=1.0):
     """(values [..., k], indices [..., k], rest [...]) of the k largest logits of every row (see ``convlogic_b200.top_logits``)."""
-    return native().top_logits(x, k, temperature)
+    return native().top_logits_raw(x, k, temperature)
 
 
 def distill_fwd(scores, values, indices, rest=None, weight=None, temperature=1.0, reduction="mean"):

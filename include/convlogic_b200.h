@@ -442,7 +442,7 @@ int clb_top_logits(const void *x, int64_t row_stride, float *values, int64_t *in
  * reduction: CLB_REDUCE_NONE (loss [rows]), CLB_REDUCE_MEAN (loss [1], the sum divided by rows) or CLB_REDUCE_SUM (loss [1]); zero rows add up to zero.
  * The forward leaves stats [rows][2] and listed [rows][k] for the backward, and writes d loss / d scores for an upstream gradient of one into grad, from
  * the scores that it holds for the loss, unless grad is NULL.
- * scratch: clb_distill_scratch_bytes; not needed for CLB_REDUCE_NONE.  1 <= k <= CLB_TOP_MAX.
+ * scratch: clb_distill_scratch_bytes, 8-byte aligned; not needed for CLB_REDUCE_NONE.  1 <= k <= CLB_TOP_MAX.
  * clb_distill_bwd: grad = upstream * d loss / d scores; upstream is one float, or one for each row (upstream_per_row).  unit_done: the forward has written
  * grad and nothing has changed it; where *upstream is 1, it is left as it is (not with upstream_per_row). */
 #define CLB_REDUCE_NONE 0

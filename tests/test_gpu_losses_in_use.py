@@ -3,6 +3,9 @@
 import pytest
 import torch
 
+from oracle import loss_oracle
+from tests.test_gpu_losses import check_grad, check_loss
+
 pytestmark = pytest.mark.gpu
 
 
@@ -74,7 +77,7 @@ def test_a_step_adds_to_the_gradients_of_a_bucket():
     with pytest.raises(RuntimeError, match="direct"):
         cb.balance_loss(w)
     with torch.no_grad():
-        assert int(cb.balance_loss(w.detach())[1].sum()) == 400     # the counts alone are no gradient
+        assert int(cb.balance_loss(w)[1].sum()) == 400              # the counts alone are no gradient
     bucket.direct(False)
     cb.balance_loss(w)
 
@@ -287,6 +290,8 @@ def test_what_torch_puts_around_a_call():
             call(fwad.make_dual(x, torch.ones_like(x)))
         with pytest.raises(RuntimeError):
             torch.func.grad(call)(x)
+    lists = torch.jit.trace(lambda s: tuple(cb.top_logits(s, 5)[:3]), (x,), check_trace=False)
+    assert all(torch.equal(p, q) for p, q in zip(lists(other), cb.top_logits(other, 5)[:3]))
     # hooks of saved tensors see what a call keeps
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.cuda()):
         y = x.clone().requires_grad_(True)
@@ -358,3 +363,74 @@ def test_every_launch_is_traced(n, v):
     names = _lib.trace_report()
     _lib.trace(False)
     assert counted > 0 and sum(c for c, _ in names.values()) == counted, names
+
+
+def test_a_million_rows():
+    """More rows than one block adds up.  Terms of one size: each row's loss is within 2e-4 of its own, and so is their mean; 64 bits add them."""
+    import convlogic_b200 as cb
+
+    x, teacher = torch.randn(1000003, 5, device="cuda"), torch.randn(1000003, 5, device="cuda")
+    top = cb.top_logits(teacher, 2)
+    rows = cb.distillation_loss(x, top, reduction="none")
+    total = rows.double().sum()
+    for how, want in (("sum", total), ("mean", total / 1000003)):
+        got = cb.distillation_loss(x, top, reduction=how)
+        # rows are rounded to 2^-24 of their size before they are added; the mean's are scaled by a rounded divisor (2^-24) before that
+        assert abs(float(got) - float(want)) <= 4 * 2.0 ** -24 * float(want)
+    loss, counts = cb.balance_loss(x, 2)
+    assert int(counts.sum()) == 2 * 1000003
+    p = torch.softmax(x.double(), 1)
+    want = 5 * (counts.double() / (2 * 1000003) * p.mean(0)).sum()
+    assert abs(float(loss) - float(want)) <= 5e-5 * float(want)
+
+
+def test_offsets_beyond_32_bits():
+    """The last rows of 4.8e9 scores."""
+    import convlogic_b200 as cb
+
+    n, v = 40000, 120001
+    x = torch.empty(n, v, dtype=torch.bfloat16, device="cuda")
+    for part in x.split(4000):
+        part.normal_(0.0, 3.0)
+    top = cb.top_logits(x, 3)
+    tail = cb.top_logits(x[-100:], 3)
+    assert all(torch.equal(a[-100:], b) for a, b in zip(top[:3], tail[:3]))
+    # (those rows begin elsewhere in their 16-byte pieces than the same rows alone, so that sums have another order: held to the definition in 64 bits)
+    up = torch.rand(n, device="cuda")
+    lists = (top.values.roll(1, 1), top.indices, top.rest)
+    last = [t[-100:] for t in lists]
+    a = x.requires_grad_(True)
+    loss = cb.distillation_loss(a, lists, reduction="none")
+    (grad,) = torch.autograd.grad(loss, a, up)
+    want = loss_oracle.distillation(x[-100:], *last, None, 1.0, "none", up[-100:])
+    check_loss(loss.detach()[-100:], want["loss"], want["loss_scale"])
+    check_grad(grad[-100:], want["grad"], want["grad_scale"], x.dtype)
+    del grad, loss
+    (grad,) = torch.autograd.grad(cb.distillation_loss(a, lists, reduction="sum"), a)
+    want = loss_oracle.distillation(x[-100:], *last, None, 1.0, "sum")
+    check_grad(grad[-100:], want["grad"], want["grad_scale"], x.dtype)
+    del grad
+    # columns of a wide tensor: rows at a distance of 120001
+    y = x.detach()[:, 119990:]
+    assert torch.equal(cb.top_logits(y, 4).indices[-5:], cb.top_logits(y[-5:].clone(), 4).indices)
+    assert torch.equal(cb.balance_loss(y[-100:])[1], cb.balance_loss(y[-100:].clone())[1])
+
+
+def test_a_tensor_of_another_stream_and_lists_in_flight():
+    """Lists made on a side stream are waited for as any tensor is; the loss's own tensors live as long as its work."""
+    import convlogic_b200 as cb
+
+    x, teacher = _scores(200, 5000).requires_grad_(True), _scores(200, 5000, seed=1)
+    want = torch.autograd.grad(cb.distillation_loss(x, cb.top_logits(teacher, 20)), x)[0]
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(20):
+        with torch.cuda.stream(side):
+            top = cb.top_logits(teacher, 20)
+        torch.cuda.current_stream().wait_stream(side)
+        for t in top[:3]:
+            t.record_stream(torch.cuda.current_stream())
+        loss = cb.distillation_loss(x, top)
+        del top
+        got = torch.autograd.grad(loss, x)[0]
+        assert torch.equal(got, want)
