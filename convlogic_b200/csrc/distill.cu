@@ -380,7 +380,8 @@ __global__ void __launch_bounds__(TH, 1024 / TH)
             for (int i = 0; i < EACH; ++i)
                 if (next.cls[i] >= 0) {
                     const int at = place(x + r * a.stride, next.cls[i]);
-                    twice = twice || ((atomicOr(&table[at >> 5], 1u << (at & 31)) >> (at & 31)) & 1);
+                    const uint32_t before = atomicOr(&table[at >> 5], 1u << (at & 31));
+                    twice = twice || ((before >> (at & 31)) & 1);
                 }
             return (bool)__any_sync(0xffffffffu, twice);
         };
@@ -641,6 +642,8 @@ DistillArgs make_args(int64_t rows, int64_t classes, int64_t row_stride, int k, 
             (float)(reduction == CLB_REDUCE_MEAN && rows > 0 ? temperature / (double)rows : temperature)};
 }
 
+constexpr long long kMostBlocks = 1 << 16; // then they take one row after another
+
 struct FwdPointers {
     const float *values;
     const int64_t *indices;
@@ -654,7 +657,7 @@ cudaError_t launch_fwd(const T *x, const FwdPointers &p, T *grad, DistillArgs a,
     const int cluster = 1 << ranks_log;
     a.ranks_log = ranks_log, a.chunks = (int)((pieces + (long long)cluster * TH * NV - 1) / ((long long)cluster * TH * NV));
     constexpr int BLOCK = TH <= 32 ? 256 : TH, TEAMS = BLOCK / TH;
-    const long long groups = (a.rows + TEAMS - 1) / TEAMS, most = (1 << 20) / cluster;
+    const long long groups = (a.rows + TEAMS - 1) / TEAMS, most = kMostBlocks / cluster;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)((groups < most ? groups : most) * cluster)), cfg.blockDim = dim3(BLOCK), cfg.stream = st;
     cudaLaunchAttribute attr[1];

@@ -479,7 +479,7 @@ extern "C" int clb_top_logits(const void *x, int64_t row_stride, float *values, 
         TopArgs a{row_stride, rows, (int)classes, k, segments_of<T>(pieces), (float)temperature, (float)(1.4426950408889634 / temperature)};
         u64 *const places = (u64 *)scratch;
         ExpSum *const sums = (ExpSum *)(places + (a.segments > 1 ? rows * a.segments * k : 0));
-        auto blocks = [](long long n) { return (unsigned)(n < (1 << 20) ? n : (1 << 20)); };
+        auto blocks = [](long long n) { return (unsigned)(n < (1 << 16) ? n : (1 << 16)); }; // (then they take one row after another)
         if (classes <= 4 * kFew) {
             const int lanes = classes <= kFew ? 1 : classes <= 2 * kFew ? 2 : 4;
             const unsigned n = blocks((rows * lanes + kBlock - 1) / kBlock);

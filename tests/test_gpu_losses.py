@@ -210,6 +210,64 @@ def test_distillation_of_odd_lists_and_masked_rows(v, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n,v,k", [(64, 2049, 5), (2500, 2500, 20), (1300, 4100, 128), (700, 8200, 64), (1300, 11000, 3), (700, 20011, 64), (310, 70003, 33), (310, 131071, 64), (160, 140003, 100)])
+def test_many_long_rows(n, v, k, dtype):
+    """More rows than blocks, so that a block's tables serve one row after another.  The rows compared: the first of every block, some of its second and third,
+    the last ones; among them rows with classes listed twice, missing entries, masked scores, weight zero and NaN."""
+    import convlogic_b200 as cb
+
+    inf, nan = math.inf, math.nan
+    g = torch.Generator(device="cuda").manual_seed(n + v)
+    x = (torch.randn(n, v, device="cuda", generator=g) * 3).to(dtype)
+    values, indices = torch.topk(x.float() + torch.randn(n, v, device="cuda", generator=g), k, 1)
+    rest = torch.rand(n, device="cuda", generator=g) * 3
+    weight = torch.rand(n, device="cuda", generator=g) + 0.5
+    row = torch.arange(n, device="cuda")
+    indices[row % 5 == 1, k // 2] = indices[row % 5 == 1, 0]
+    indices[row % 7 == 2, 0] = -1
+    x[row % 6 == 3, v // 3:] = -inf
+    weight[row % 9 == 4] = 0.0
+    x[row % 18 == 4, 0] = nan
+    x[row % 23 == 5] = -inf
+    values[row % 29 == 6], rest[row % 29 == 6] = -inf, -inf
+    rest[row % 11 == 7] = -inf
+    up = torch.rand(n, device="cuda", generator=g) + 0.5
+    some = torch.cat([row[:24], row[n // 2 - 12:n // 2 + 12], row[-24:]])
+    want = loss_oracle.distillation(x[some], values[some], indices[some], rest[some], weight[some], 1.5, "none", up[some])
+    x.requires_grad_(True)
+    loss = cb.distillation_loss(x, (values, indices, rest), 1.5, weight, "none")
+    check_loss(loss.detach()[some], want["loss"], want["loss_scale"])
+    check_grad(torch.autograd.grad(loss, x, up)[0][some], want["grad"], want["grad_scale"], dtype)
+    # the forward's own gradient, and the sum; a row whose loss is infinite (its student has masked what the teacher knows) is left out of that
+    loss = cb.distillation_loss(x, (values, indices, rest), 1.5, weight, "sum")
+    want = loss_oracle.distillation(x[some], values[some], indices[some], rest[some], weight[some], 1.5, "sum")
+    check_grad(torch.autograd.grad(loss, x)[0][some], want["grad"], want["grad_scale"], dtype)
+
+
+@pytest.mark.parametrize("n,v,k", [(67000, 5300, 9), (67000, 12000, 5), (530000, 1500, 5), (530000, 700, 40), (1100000, 300, 4), (2200000, 100, 3), (4300000, 9, 3), (17000000, 3, 1)])
+def test_more_rows_than_a_grid_has_teams(n, v, k):
+    """The first, the last and the first of the second turn."""
+    import convlogic_b200 as cb
+
+    x = torch.empty(n, v, dtype=torch.bfloat16, device="cuda")
+    for part in x.split(max(1, (1 << 27) // v)):
+        part.normal_(0.0, 3.0)
+    top = cb.top_logits(x, k, 1.5)
+    turns = [t for t in (1 << 16, 1 << 19, 1 << 20, 1 << 21, 1 << 22, 1 << 24) if t + 8 < n]
+    some = torch.cat([torch.arange(8)] + [torch.arange(t - 8, t + 8) for t in turns] + [torch.arange(n - 8, n)]).cuda()
+    values, indices, rest = loss_oracle.top_logits(x[some], k, 1.5)
+    assert torch.equal(top.values[some].cpu().double(), values) and torch.equal(top.indices[some].cpu(), indices)
+    assert ((top.rest[some].cpu().double() - rest).abs() <= 2 * EPS + 4 * 2.0 ** -24 * rest.abs()).all()
+    lists = (top.values.roll(1, 1), top.indices, top.rest)
+    want = loss_oracle.distillation(x[some], *(t[some] for t in lists), None, 1.5, "none", 1.0)
+    x.requires_grad_(True)
+    loss = cb.distillation_loss(x, lists, 1.5, None, "none")
+    check_loss(loss.detach()[some], want["loss"], want["loss_scale"])
+    check_grad(torch.autograd.grad(loss, x, torch.ones_like(loss))[0][some], want["grad"], want["grad_scale"], x.dtype)
+    check_grad(torch.autograd.grad(cb.distillation_loss(x, lists, 1.5, None, "sum"), x)[0][some], want["grad"], want["grad_scale"], x.dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("v", [10, 1000, 20000, 140000])
 def test_rows_that_count_for_nothing(v, dtype):
     """Weight zero, no teacher, no student: nothing is added and the gradient is zero, whatever stands there; NaN elsewhere stays in its row."""
