@@ -21,6 +21,7 @@ using namespace clb_host;
 namespace {
 
 template <int NC> constexpr int kThreads = NC > 16 ? 128 : 256; // of a block (32 columns a lane: what four warps' sums take of shared memory)
+template <int G, int NC> constexpr int kResident = NC > 16 || G == 1 ? 4 : 3; // blocks an SM, which is how many are launched
 constexpr float kLog2e = 1.44269504f;
 
 // The columns of lane t of G: pieces of 16 bytes (VEC: rows at multiples of 16 bytes, whole pieces), or every G-th column.  Ascending either way.
@@ -79,7 +80,7 @@ template <int G, int NC> __device__ __forceinline__ float soft_max(float (&v)[NC
 // Choices are found among the logits themselves: the largest, the first of equal ones, then it becomes -inf, which is never chosen (NaN counts as +inf).
 // Their counts are bytes in a lane's registers, handed to the block every 255 rows.
 template <typename T, int G, int NC, bool VEC>
-__global__ void __launch_bounds__(kThreads<NC>) balance_fwd_kernel(const T *__restrict__ x, long long stride, const uint8_t *__restrict__ keep,
+__global__ void __launch_bounds__(kThreads<NC>, kResident<G, NC>) balance_fwd_kernel(const T *__restrict__ x, long long stride, const uint8_t *__restrict__ keep,
                                                                float *__restrict__ sums, int *__restrict__ counts, int *__restrict__ kept, int rows, int experts,
                                                                int k)
 {
@@ -218,7 +219,7 @@ __global__ void __launch_bounds__(1024) balance_finish_kernel(const float *__res
 }
 
 template <typename T, int G, int NC, bool VEC>
-__global__ void __launch_bounds__(kThreads<NC>) balance_bwd_kernel(const T *__restrict__ x, long long stride, const uint8_t *__restrict__ keep,
+__global__ void __launch_bounds__(kThreads<NC>, kResident<G, NC>) balance_bwd_kernel(const T *__restrict__ x, long long stride, const uint8_t *__restrict__ keep,
                                                                const float *__restrict__ share, const float *__restrict__ up, T *__restrict__ gx, int rows,
                                                                int experts)
 {
@@ -283,17 +284,15 @@ template <typename F> void with_team(int64_t experts, F &&f)
     else if (experts <= 512) f(integral_constant<int, 32>(), integral_constant<int, 16>());
     else f(integral_constant<int, 32>(), integral_constant<int, 32>());
 }
-int teams_of(int64_t experts) // of a block
-{
-    int n = 0;
-    with_team(experts, [&](auto G, auto NC) { n = kThreads<decltype(NC)::value> / decltype(G)::value; });
-    return n;
-}
-// Blocks of the forward pass: up to four an SM, and sums of at most 512 KB for the one block that finishes.
+// Blocks of the forward pass: those that are resident, and sums of at most 512 KB for the one block that finishes.  (Of 148 SMs: what the scratch is for.)
 int balance_blocks(int64_t rows, int64_t experts)
 {
-    const int64_t teams = teams_of(experts), most = std::min<int64_t>(4 * 148, std::max<int64_t>(64, 65536 / experts));
-    return (int)std::min<int64_t>((rows + teams - 1) / teams, most);
+    int64_t n = 0;
+    with_team(experts, [&](auto G, auto NC) {
+        const int64_t teams = kThreads<decltype(NC)::value> / decltype(G)::value;
+        n = std::min<int64_t>((rows + teams - 1) / teams, std::min<int64_t>(148 * kResident<decltype(G)::value, decltype(NC)::value>, std::max<int64_t>(64, 65536 / experts)));
+    });
+    return (int)n;
 }
 template <typename T> bool whole_pieces(const void *x, int64_t stride, int64_t experts)
 {
@@ -353,7 +352,7 @@ extern "C" int clb_balance_bwd(const void *x, int64_t row_stride, const uint8_t 
         with_team(experts, [&](auto G, auto NC) {
             constexpr int LANES = decltype(G)::value;
             const int64_t teams = kThreads<decltype(NC)::value> / LANES;
-            const int blocks = (int)std::min<int64_t>((rows + teams - 1) / teams, 6 * (int64_t)sm_count());
+            const int blocks = (int)std::min<int64_t>((rows + teams - 1) / teams, kResident<LANES, decltype(NC)::value> * (int64_t)sm_count());
             auto go = [&](auto vec) {
                 constexpr bool VEC = decltype(vec)::value;
                 CLB_TRACED("balance_bwd_kernel", st,
