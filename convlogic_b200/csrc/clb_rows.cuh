@@ -133,7 +133,6 @@ template <typename T> struct RowPieces {
             }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
-    __device__ __forceinline__ uint4 piece(int j) const { return whole(j) ? __ldg(reinterpret_cast<const uint4 *>(row + first(j))) : edge(j); }
     // pieces j, j + step, ...: the whole ones are asked for before anything waits.  LAST: not read again
     template <int NV, bool LAST = true> __device__ __forceinline__ void load(uint4 (&q)[NV], int j, int step) const
     {

@@ -7,7 +7,7 @@
 //   1. The k-th largest of the threads' own maxima, rounded down to 16 bits of its order, is a bound that at least k values reach, and few more: with 256 maxima
 //      of 64 values about 75 for k = 64.  One warp finds it by bisection.
 //   2. The values that reach the bound go to a list in shared memory; the others are added up as exponentials with respect to the bound.
-//   3. Each value's place in the list is the number of those above it; (value, index) are one 64-bit number, so that no two are alike.
+//   3. Each value's place in the list is the number of those above it, equal ones by index.
 // Values that tie in great numbers, more than the list holds, take a second way: bisection over all values for the k-th largest, then over the indices of those
 // that equal it.  Segments leave their k largest and the sum of their others; a block a row puts them together.
 #include "clb_rows.cuh"
@@ -83,10 +83,59 @@ template <int TH> __device__ __forceinline__ ExpSum team_merge(ExpSum s, ExpSum 
     return lanes_merge<TH / 32>(box[threadIdx.x % (TH / 32)], c);
 }
 
-// the place of each of `count` candidates among them, handed to `f`
-template <int TH, typename F> __device__ __forceinline__ void ranked(const u64 *cand, int count, int t, F &&f)
+// Candidates of a team, as 32-bit numbers of their order, 0 behind the last one up to a multiple of four.  Values of 16 bits share theirs with the class (counted
+// from the segment's first), so that no two are alike; for floats, which tie seldom, the class stands beside it and is asked for only where two are alike.
+template <typename T, int CAP> struct Candidates {
+    static constexpr bool kShared = sizeof(T) == 2;
+    uint4 four[CAP / 4 + 1];
+    uint32_t cls[kShared ? 1 : CAP];
+    __device__ __forceinline__ uint32_t *one() { return reinterpret_cast<uint32_t *>(four); }
+    __device__ __forceinline__ void put(int n, float v, int c) // c: from the segment's first class
+    {
+        if constexpr (kShared) {
+            const uint32_t b = raw_bits(from_f<T>(v)), k = v != v ? 0xffffu : v == 0.f ? 0x8000u : b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+            one()[n] = k << 16 | (0xffffu - (uint32_t)c);
+        } else
+            one()[n] = order_key(v), cls[n] = c;
+    }
+    __device__ __forceinline__ float value(uint32_t o) const
+    {
+        if constexpr (kShared) {
+            const uint32_t k = o >> 16, b = k == 0xffffu ? 0x7fffu : k & 0x8000u ? k & 0x7fffu : ~k & 0xffffu;
+            float f[2];
+            two_values<T>(b, f);
+            return f[0];
+        } else
+            return value_of(o);
+    }
+    __device__ __forceinline__ int class_at(int n) const
+    {
+        if constexpr (kShared) return (int)(0xffffu - (reinterpret_cast<const uint32_t *>(four)[n] & 0xffffu));
+        else return (int)cls[n];
+    }
+};
+// the place of each of `count` candidates among them, its value and class handed to `f`
+template <int TH, typename T, int CAP, typename F> __device__ __forceinline__ void ranked(Candidates<T, CAP> &c, int count, int t, F &&f)
 {
     for (int i = t; i < count; i += TH) {
+        const uint32_t mine = c.one()[i];
+        const int cls = c.class_at(i);
+        int above = 0, same = 0;
+#pragma unroll 4
+        for (int j = 0; j < count; j += 4) {
+            const uint4 q = c.four[j / 4];
+            above += (q.x > mine) + (q.y > mine) + (q.z > mine) + (q.w > mine);
+            if (!c.kShared) same += (q.x == mine) + (q.y == mine) + (q.z == mine) + (q.w == mine);
+        }
+        if (same > 1)
+            for (int j = 0; j < count; ++j) above += c.one()[j] == mine && c.class_at(j) < cls;
+        f(above, c.value(mine), cls);
+    }
+}
+// the same of 64-bit places
+template <typename F> __device__ __forceinline__ void ranked_places(const u64 *cand, int count, int t, F &&f)
+{
+    for (int i = t; i < count; i += kBlock) {
         const u64 mine = cand[i];
         int above = 0;
 #pragma unroll 4
@@ -105,13 +154,15 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
 {
     constexpr int TEAMS = TH == 32 ? kBlock / TH : 1, EV = kPiece<T>, CAP = TH == 32 ? 256 : 512;
     static_assert(NV % SUB == 0 || 2 * NV == SUB, "groups of whole or half pieces");
-    __shared__ __align__(16) u64 cand_all[TEAMS][CAP + 2];
-    __shared__ uint32_t keys_all[TEAMS][TH * SUB], extra_all[TEAMS][CAP];
+    __shared__ Candidates<T, CAP> cand_all[TEAMS];
+    __shared__ uint32_t keys_all[TEAMS][TH * SUB];
+    __shared__ float extra_all[TEAMS][CAP];
     __shared__ int count_all[TEAMS], box[TH / 32 + 1];
     __shared__ uint32_t bound_all[TEAMS];
     __shared__ ExpSum sum_box[TH / 32];
+    __shared__ float l_box[TH / 32];
     const int t = threadIdx.x % TH, team = threadIdx.x / TH;
-    u64 *const cand = cand_all[team];
+    Candidates<T, CAP> &cand = cand_all[team];
     const long long items = a.rows * a.segments;
     for (long long item = (long long)blockIdx.x * TEAMS + team; item < items; item += (long long)gridDim.x * TEAMS) {
         const long long r = a.segments == 1 ? item : item / a.segments;
@@ -149,6 +200,8 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
             keys_all[team][s * TH + t] = word_key<T>(top);
         }
         if (t == 0) count_all[team] = 0;
+        if (TH > 32)
+            for (int i = t; i < CAP / 4 + 1; i += TH) cand.four[i] = make_uint4(0, 0, 0, 0); // (what is behind the list's end)
         team_sync<TH>();
         if (t < 32) {
             uint32_t key[TH * SUB / 32];
@@ -163,12 +216,11 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
         const bool few = bound == kMasked + 1;
         const float reach = value_of(bound);
         // ---- 2: candidates, and the sum of the others
+        const int own_first = base == 0 ? 0 : row.first(base); // the segment's first class
         auto push = [&](float v, int cls) {
             const int n = atomicAdd(&count_all[team], 1);
-            if (n < CAP) cand[n] = place_of(order_key(v), cls);
+            if (n < CAP) cand.put(n, v, cls - own_first);
         };
-        const int first_class = max(0, row.first(base));
-        const int own_first = base == 0 ? 0 : first_class; // the segment's first class
         const ExpRef er = exp_ref(reach, a.c);
         float l = 0.f;
         uint32_t hits = 0; // pieces with a candidate
@@ -203,23 +255,48 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
                     }
             hits = 0;
         }
-        while (hits) { // read once more: a warp has as many turns as its lanes have such pieces at most, one or two, not one for every piece
+        while (hits) { // a warp has as many turns as its lanes have such pieces at most, one or two, not one for every piece
             const int i = __ffs(hits) - 1;
             hits &= hits - 1;
-            const uint4 p = row.piece(base + i * TH + t);
-            const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+            uint4 p = raw[0];
 #pragma unroll
-            for (int e = 0; e < EV; ++e) {
+            for (int n = 1; n < NV; ++n) {
+                p.x = n == i ? raw[n].x : p.x, p.y = n == i ? raw[n].y : p.y;
+                p.z = n == i ? raw[n].z : p.z, p.w = n == i ? raw[n].w : p.w;
+            }
+            const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+            const int first = row.first(base + i * TH + t);
+            uint32_t which = 0;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
                 float f[Word<T>::n];
-                Word<T>::get(w[Word<T>::n == 1 ? e & 3 : e >> 1], f);
-                const float v = f[Word<T>::n == 1 ? 0 : e & 1];
-                const int cls = class_of(i, e);
-                if (cls >= 0 && (!(v < reach) || (few && cls < own_first + a.k))) push(v, cls);
+                Word<T>::get(w[q], f);
+#pragma unroll
+                for (int z = 0; z < Word<T>::n; ++z) {
+                    const int e = q * Word<T>::n + z;
+                    which |= (uint32_t)!(f[z] < reach) << e;
+                    if (few && first + e >= 0 && first + e < min(a.classes, own_first + a.k)) which |= 1u << e;
+                }
+            }
+            while (which) {
+                const int e = __ffs(which) - 1;
+                which &= which - 1;
+                const int at = Word<T>::n == 1 ? e : e >> 1;
+                const uint32_t word = at == 0 ? w[0] : at == 1 ? w[1] : at == 2 ? w[2] : w[3];
+                float f[Word<T>::n];
+                Word<T>::get(word, f);
+                push(Word<T>::n == 2 && (e & 1) ? f[Word<T>::n - 1] : f[0], first + e);
             }
         }
-        l *= er.fix;
+        l = lanes_sum<32>(l * er.fix);
+        if (TH > 32 && (t & 31) == 0) l_box[t >> 5] = l;
         team_sync<TH>();
         int count = count_all[team];
+        if (TH > 32) {
+            l = 0.f;
+#pragma unroll
+            for (int w = 0; w < TH / 32; ++w) l += l_box[w];
+        }
         // f(value, class) for each of the thread's values; code of its own, as what follows is rare (a rotation: no register is named by a number that varies)
         auto for_each = [&](auto f) {
 #pragma unroll 1
@@ -258,46 +335,53 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
             team_sync<TH>();
             count = count_all[team];
         }
-        if (t == 0) cand[count] = cand[count + 1] = 0;
-        team_sync<TH>();
+        if (TH == 32 || overflow) {
+            if (t < 4) cand.one()[count + t] = 0;
+            team_sync<TH>();
+        }
         // ---- 3: their places
-        ExpSum others{reach, l};
-        bool inf = false;
         const long long at = item * a.k;
         uint32_t *const kth_box = keys_all[team];
-        ranked<TH>(cand, count, t, [&](int rank, u64 place) {
-            const uint32_t key = (uint32_t)(place >> 32);
+        ranked<TH>(cand, count, t, [&](int rank, float v, int c) {
+            const int cls = own_first + c;
             if (rank < a.k) {
-                if (a.segments == 1) values[at + rank] = value_of(key), indices[at + rank] = index_of(place);
-                else places[at + rank] = place;
-                if (rank == a.k - 1) kth_box[0] = key, kth_box[1] = (uint32_t)place;
+                if (a.segments == 1) values[at + rank] = v, indices[at + rank] = cls;
+                else places[at + rank] = place_of(order_key(v), cls);
+                if (rank == a.k - 1) kth_box[0] = order_key(v), kth_box[1] = cls;
             } else
-                extra_all[team][rank - a.k] = key;
+                extra_all[team][rank - a.k] = v;
         });
-        team_sync<TH>();
-        for (int i = t; i < count - a.k; i += TH) { // in the order of their places, whatever the order in which they came to the list
-            const float v = value_of(extra_all[team][i]);
-            if (v == INFINITY) inf = true;
-            else others = merge(others, single(v), a.c);
-        }
         if (a.segments > 1)
             for (int n = count + t; n < a.k; n += TH) places[at + n] = 0; // a last segment of few classes
-        others = team_merge<TH>(others, sum_box, a.c);
-        if (overflow || er.far || !(reach < INFINITY) || !(others.l > 1e-20f)) {
-            // the bound is no reference for the others, or they are not all counted: once more, with respect to their own largest
-            const u64 kth = count >= a.k ? ((u64)kth_box[0] << 32) | kth_box[1] : 0;
-            others = ExpSum{-INFINITY, 0.f}, inf = false;
+        team_sync<TH>();
+        auto finish = [&](ExpSum others) {
+            if (a.segments == 1) rest[r] = others.m / a.temperature + logf(others.l);
+            else sums[item] = others;
+        };
+        if (overflow || er.far || !(reach < INFINITY) || (!(l > 1e-20f) && count <= a.k)) {
+            // the bound is no reference for the others (they are far below it), or they are not all counted: once more, with respect to their own largest
+            const u64 kth = count >= a.k ? place_of(kth_box[0], kth_box[1]) : 0;
+            ExpSum others{-INFINITY, 0.f};
+            bool inf = false;
             for_each([&](float v, int cls) {
                 if (place_of(order_key(v), cls) >= kth) return;
                 if (v == INFINITY) inf = true;
                 else others = merge(others, single(v), a.c);
             });
             others = team_merge<TH>(others, sum_box, a.c);
-        }
-        if (team_count<TH>(inf, box) && others.l == others.l) others = ExpSum{INFINITY, 1.f};
-        if (t == 0) {
-            if (a.segments == 1) rest[r] = others.m / a.temperature + logf(others.l);
-            else sums[item] = others;
+            if (team_count<TH>(inf, box) && others.l == others.l) others = ExpSum{INFINITY, 1.f};
+            if (t == 0) finish(others);
+        } else if (t < 32) {
+            ExpSum others{reach, t == 0 ? l : 0.f};
+            bool inf = false;
+            for (int i = t; i < count - a.k; i += 32) { // in the order of their places, whatever the order in which they came to the list
+                const float v = extra_all[team][i];
+                if (v == INFINITY) inf = true;
+                else others = merge(others, single(v), a.c);
+            }
+            others = lanes_merge<32>(others, a.c);
+            if (__any_sync(0xffffffffu, inf) && others.l == others.l) others = ExpSum{INFINITY, 1.f};
+            if (t == 0) finish(others);
         }
         team_sync<TH>(); // the tables are used again
     }
@@ -396,7 +480,7 @@ __global__ void __launch_bounds__(kBlock) top_merge_kernel(const u64 *__restrict
         if (count <= CAP) {
             if (t == 0) cand[count] = cand[count + 1] = 0;
             __syncthreads();
-            ranked<kBlock>(cand, count, t, [&](int rank, u64 place) {
+            ranked_places(cand, count, t, [&](int rank, u64 place) {
                 if (rank >= a.k) return;
                 values[r * a.k + rank] = value_of((uint32_t)(place >> 32)), indices[r * a.k + rank] = index_of(place);
                 if (rank == a.k - 1) kth_box = place;
