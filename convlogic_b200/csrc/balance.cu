@@ -11,12 +11,15 @@
 // all its rows: no atomics, the same sums every time.  Both passes are bound by HBM (or by the L2 where the logits fit it); the backward pass goes
 // through the rows from the last one on, which is what the L2 still holds.
 #include <algorithm>
+#include <cooperative_groups.h>
 #include <type_traits>
 
 #include "clb_rows.cuh"
 
 using namespace clb;
 using namespace clb_host;
+
+namespace cg = cooperative_groups;
 
 namespace {
 
@@ -77,9 +80,116 @@ template <int G, int NC> __device__ __forceinline__ float soft_max(float (&v)[NC
     return l;
 }
 
-// Choices are found among the logits themselves: the largest, the first of equal ones, then it becomes -inf, which is never chosen (NaN counts as +inf).
-// Their counts are bytes in a lane's registers, handed to the block every 255 rows.
-template <typename T, int G, int NC, bool VEC>
+// Descending, by Batcher's odd-even merges
+template <int N> __device__ __forceinline__ void sort_down(float (&w)[N])
+{
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int d = p; d >= 1; d /= 2)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i >= d % p && (i - d % p) / d % 2 == 0 && i + d < N && i / (2 * p) == (i + d) / (2 * p)) {
+                    const float hi = fmaxf(w[i], w[i + d]);
+                    w[i + d] = fminf(w[i], w[i + d]), w[i] = hi;
+                }
+}
+// Adds the k largest of a row to the bytes of `own`: equal ones by column, never one of -inf.  One after the other: the largest, the first of equal ones, then it
+// becomes -inf.
+template <typename T, int G, int NC, bool VEC> __device__ __forceinline__ void choose_in_turn(float (&u)[NC], uint32_t (&own)[NC / 4], int t, int k)
+{
+    for (int n = 0; n < k; ++n) {
+        float best = u[0];
+        int at = 0;
+#pragma unroll
+        for (int i = 1; i < NC; ++i)
+            if (u[i] > best) best = u[i], at = i;
+        float top = best;
+        if (G > 1) {
+            top = lanes_max<G>(best);
+            const int col = column<T, G, NC, VEC>(at, t);
+            int first = best == top ? col : 0x7fffffff;
+#pragma unroll
+            for (int o = G / 2; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
+            if (first != col) at = -1;
+        }
+        if (top == -INFINITY) at = -1; // nothing is left to choose
+#pragma unroll
+        for (int i = 0; i < NC / 4; ++i) own[i] += at >> 2 == i ? 1u << ((at & 3) * 8) : 0u;
+        if (n + 1 < k)
+#pragma unroll
+            for (int i = 0; i < NC; ++i) u[i] = i == at ? -INFINITY : u[i];
+    }
+}
+// The same by the k-th largest value: every lane sorts its own, the team takes the first of a lane's k times.  What is above it is chosen, then as many of
+// those that equal it as are missing.
+template <typename T, int G, int NC, bool VEC> __device__ __forceinline__ void choose_sorted(const float (&u)[NC], uint32_t (&own)[NC / 4], int t, int k)
+{
+    const int lane = threadIdx.x & 31;
+    float w[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) w[i] = u[i];
+    sort_down(w);
+    float bound = w[0];
+    if (G == 1) {
+#pragma unroll
+        for (int i = 1; i < NC; ++i) bound = i == k - 1 ? w[i] : bound;
+    } else {
+        constexpr uint32_t kTeam = G == 32 ? 0xffffffffu : (1u << G) - 1;
+        for (int n = 0; n < k; ++n) {
+            bound = lanes_max<G>(w[0]);
+            const uint32_t holders = __ballot_sync(0xffffffffu, w[0] == bound) & (kTeam << (lane & ~(G - 1)));
+            const bool taken = (holders & (0u - holders)) == 1u << lane;
+#pragma unroll
+            for (int i = 0; i < NC - 1; ++i) w[i] = taken ? w[i + 1] : w[i];
+            w[NC - 1] = taken ? -INFINITY : w[NC - 1];
+        }
+    }
+    bound = fmaxf(bound, -3.402823466e38f);
+    int above = 0, equal = 0;
+#pragma unroll
+    for (int i = 0; i < NC; ++i) above += u[i] > bound, equal += u[i] == bound;
+    if (G > 1) {
+        int both = above | equal << 16;
+#pragma unroll
+        for (int o = G / 2; o > 0; o >>= 1) both += __shfl_xor_sync(0xffffffffu, both, o);
+        above = both & 0xffff, equal = both >> 16;
+    }
+    int missing = min(k - above, equal);
+    if (G > 1 && !__any_sync(0xffffffffu, missing < equal)) {
+#pragma unroll
+        for (int i = 0; i < NC; ++i) own[i / 4] += u[i] >= bound ? 1u << (i % 4 * 8) : 0u;
+        return;
+    }
+    // columns ascend with a lane's i: each piece of 16 bytes (each column) after those of the lanes before
+    constexpr int RUN = VEC ? kPiece<T> : 1;
+#pragma unroll
+    for (int i0 = 0; i0 < NC; i0 += RUN) {
+        int here = 0, before = 0;
+#pragma unroll
+        for (int i = i0; i < i0 + RUN; ++i) here += u[i] == bound;
+        int upto = here;
+        if (G > 1) {
+#pragma unroll
+            for (int o = 1; o < G; o *= 2) {
+                const int n = __shfl_up_sync(0xffffffffu, upto, o, G);
+                upto += t >= o ? n : 0;
+            }
+            before = upto - here;
+            upto = __shfl_sync(0xffffffffu, upto, G - 1, G);
+        }
+#pragma unroll
+        for (int i = i0; i < i0 + RUN; ++i) {
+            const bool same = u[i] == bound;
+            own[i / 4] += u[i] > bound || (same && before < missing) ? 1u << (i % 4 * 8) : 0u;
+            before += same;
+        }
+        missing -= upto;
+    }
+}
+
+// A row's choices are counted as bytes in a lane's registers, handed to the block every 255 rows (NaN counts as +inf).
+template <typename T, int G, int NC, bool VEC, bool SORT>
 __global__ void __launch_bounds__(kThreads<NC>, kResident<G, NC>) balance_fwd_kernel(const T *__restrict__ x, long long stride, const uint8_t *__restrict__ keep,
                                                                float *__restrict__ sums, int *__restrict__ counts, int *__restrict__ kept, int rows, int experts,
                                                                int k)
@@ -126,28 +236,8 @@ __global__ void __launch_bounds__(kThreads<NC>, kResident<G, NC>) balance_fwd_ke
             for (int i = 0; i < NC; ++i) u[i] = u[i] != u[i] ? INFINITY : u[i];
 #pragma unroll
         for (int i = 0; i < NC; ++i) acc[i] += l != 0.f ? v[i] : 0.f;
-        for (int n = 0; n < k; ++n) {
-            float best = u[0];
-            int at = 0;
-#pragma unroll
-            for (int i = 1; i < NC; ++i)
-                if (u[i] > best) best = u[i], at = i;
-            float top = best;
-            if (G > 1) {
-                top = lanes_max<G>(best);
-                const int col = column<T, G, NC, VEC>(at, t);
-                int first = best == top ? col : 0x7fffffff;
-#pragma unroll
-                for (int o = G / 2; o > 0; o >>= 1) first = min(first, __shfl_xor_sync(0xffffffffu, first, o));
-                if (first != col) at = -1;
-            }
-            if (top == -INFINITY) at = -1; // nothing is left to choose
-#pragma unroll
-            for (int i = 0; i < NC / 4; ++i) own[i] += at >> 2 == i ? 1u << ((at & 3) * 8) : 0u;
-            if (n + 1 < k)
-#pragma unroll
-                for (int i = 0; i < NC; ++i) u[i] = i == at ? -INFINITY : u[i];
-        }
+        if constexpr (SORT) choose_sorted<T, G, NC, VEC>(u, own, t, k);
+        else choose_in_turn<T, G, NC, VEC>(u, own, t, k);
         if (++since == 255) hand_over();
     }
     hand_over();
@@ -175,7 +265,9 @@ __global__ void __launch_bounds__(kThreads<NC>, kResident<G, NC>) balance_fwd_ke
     }
 }
 
-// Adds up the blocks' sums: `per` threads an expert, each its share of the blocks in order.
+// Adds up the blocks' sums: one block, or a cluster of blocks where there are many (what a single SM takes in would be the time).  `per` threads an expert and
+// block, each its share of the sums in order, then a tree over the threads, then the cluster's blocks in order.
+constexpr int kFinishBlocks = 8;
 __global__ void __launch_bounds__(1024) balance_finish_kernel(const float *__restrict__ sums, const int *__restrict__ counts, const int *__restrict__ kept,
                                                               float *__restrict__ loss, int64_t *__restrict__ total, float *__restrict__ share, int blocks,
                                                               int experts, int per, int k)
@@ -184,19 +276,35 @@ __global__ void __launch_bounds__(1024) balance_finish_kernel(const float *__res
     __shared__ long long cs[1024];
     __shared__ double red[4][32];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int rank = blockIdx.x, ranks = gridDim.x; // one cluster
     // thread = part * experts + e: neighbours read neighbouring experts
     const int e = threadIdx.x % experts, part = threadIdx.x / experts;
     double p = 0.0;
     long long c = 0;
     if (part < per)
-        for (int b = part; b < blocks; b += per) p += sums[(long long)b * experts + e], c += counts[(long long)b * experts + e];
+        for (int b = rank * per + part; b < blocks; b += ranks * per) p += sums[(long long)b * experts + e], c += counts[(long long)b * experts + e];
     ps[threadIdx.x] = p, cs[threadIdx.x] = c;
     double m = 0.0;
-    for (int b = threadIdx.x; b < blocks; b += 1024) m += kept[b];
+    if (rank == 0)
+        for (int b = threadIdx.x; b < blocks; b += 1024) m += kept[b];
     __syncthreads();
+    for (int n = per; n > 1; n = (n + 1) / 2) { // n parts: the upper ones are added to the lower ones
+        if (part + (n + 1) / 2 < n) ps[threadIdx.x] += ps[threadIdx.x + (n + 1) / 2 * experts], cs[threadIdx.x] += cs[threadIdx.x + (n + 1) / 2 * experts];
+        __syncthreads();
+    }
+    if (ranks > 1) {
+        cluster.sync();
+        if (rank > 0) {
+            cluster.sync(); // its sums are read until here
+            return;
+        }
+    }
     p = 0.0, c = 0;
+    if (threadIdx.x < experts) p = ps[threadIdx.x], c = cs[threadIdx.x];
     if (threadIdx.x < experts)
-        for (int i = 0; i < per; ++i) p += ps[i * experts + threadIdx.x], c += cs[i * experts + threadIdx.x];
+        for (int i = 1; i < ranks; ++i) p += cluster.map_shared_rank(ps, i)[threadIdx.x], c += cluster.map_shared_rank(cs, i)[threadIdx.x];
+    if (ranks > 1) cluster.sync();
     double v[4] = {(double)c * p, (double)c, m, p};
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1)
@@ -324,18 +432,33 @@ extern "C" int clb_balance_fwd(const void *x, int64_t row_stride, const uint8_t 
         with_score_type(dtype, [&](auto t) {
             using T = decltype(t);
             with_team(experts, [&](auto G, auto NC) {
-                auto go = [&](auto vec) {
-                    constexpr bool VEC = decltype(vec)::value;
+                constexpr int LANES = decltype(G)::value, COLUMNS = decltype(NC)::value;
+                auto go = [&](auto vec, auto sort) {
+                    constexpr bool VEC = decltype(vec)::value, SORT = decltype(sort)::value;
                     CLB_TRACED("balance_fwd_kernel", st,
-                               balance_fwd_kernel<T, decltype(G)::value, decltype(NC)::value, VEC><<<blocks, kThreads<decltype(NC)::value>, 0, st>>>(
+                               balance_fwd_kernel<T, LANES, COLUMNS, VEC, SORT><<<blocks, kThreads<COLUMNS>, 0, st>>>(
                                    (const T *)x, row_stride, keep, sums, cnt, kept, (int)rows, (int)experts, k));
                 };
-                if (whole_pieces<T>(x, row_stride, experts)) go(std::true_type());
-                else go(std::false_type());
+                auto chosen = [&](auto sort) {
+                    if (whole_pieces<T>(x, row_stride, experts)) go(std::true_type(), sort);
+                    else go(std::false_type(), sort);
+                };
+                if constexpr (COLUMNS == 16) {
+                    // in turn / sorted, 16 million logits: k = 2 30 / 43 us (16 experts), 31 / 38 (128); k = 4 40 / 42, 44 / 41; k = 8 62 / 42, 71 / 48
+                    if (k >= (LANES == 1 ? 5 : 4)) return chosen(std::true_type());
+                }
+                chosen(std::false_type());
             });
         });
-    CLB_TRACED("balance_finish_kernel", st, balance_finish_kernel<<<1, 1024, 0, st>>>(sums, cnt, kept, loss, counts, share, blocks, (int)experts,
-                                                                                                  (int)(1024 / experts), k));
+    const int ranks = blocks * experts > 32768 ? kFinishBlocks : 1; // one / eight, us: 592 sums of 30 experts 7 / 8, 444 of 60 9 / 7, 256 of 256 12 / 8
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(ranks), cfg.blockDim = dim3(1024), cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = (unsigned)ranks, attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr, cfg.numAttrs = 1;
+    CLB_TRACED("balance_finish_kernel", st, cudaLaunchKernelEx(&cfg, balance_finish_kernel, (const float *)sums, (const int *)cnt, (const int *)kept, loss, counts,
+                                                               share, blocks, (int)experts, (int)(1024 / experts), k));
     return check_launch(rows > 0 ? 2 : 1);
 }
 

@@ -287,14 +287,15 @@ __device__ __forceinline__ ExpRef exp_ref(float m, float c)
 }
 template <int LANES> __device__ __forceinline__ float lanes_max(float v) // NaN is passed over
 {
-    if (LANES == 32) { // one instruction for the warp
+    if constexpr (LANES == 32) { // one instruction for the warp
         float r;
         asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
         return r;
-    }
+    } else {
 #pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
+        for (int o = LANES / 2; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+        return v;
+    }
 }
 template <int LANES> __device__ __forceinline__ float lanes_sum(float v)
 {
@@ -314,7 +315,7 @@ template <typename T, int TH, int NV> struct RowTrips {
     static constexpr int kBytes = TH * NV * 16;
     const char *first; // the thread's piece 0 of trip 0 (not to be read unless trip 0 is whole)
     int lo, hi;
-    __device__ __forceinline__ RowTrips() = default;
+    RowTrips() = default;
     __device__ __forceinline__ RowTrips(const T *row, int classes)
     {
         const int phase = (int)((reinterpret_cast<uintptr_t>(row) & 15) / sizeof(T));

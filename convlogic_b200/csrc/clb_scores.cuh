@@ -1,4 +1,4 @@
-// What the kernels on rows of scores share (distill.cu, top_logits.cu, balance.cu): element types, exponentials, block sums.
+// What the kernels on rows of scores share (distill.cu, top_logits.cu, balance.cu): element types, sums of exponentials, order.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -30,12 +30,6 @@ __device__ __forceinline__ ExpSum merge(ExpSum a, ExpSum b, float c)
     const float m = fmaxf(a.m, b.m);
     if (m == -INFINITY) return {m, a.l + b.l}; // nothing, or NaN in l
     return {m, a.l * exp_diff(a.m, m, c) + b.l * exp_diff(b.m, m, c)};
-}
-__device__ __forceinline__ ExpSum warp_merge(ExpSum s, float c)
-{
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s = merge(s, ExpSum{__shfl_xor_sync(0xffffffffu, s.m, o), __shfl_xor_sync(0xffffffffu, s.l, o)}, c);
-    return s;
 }
 
 // Order of scores as unsigned integers: larger is larger, -0 equals +0, NaN above everything; never 0 and never all ones, which stand for "before the

@@ -381,6 +381,19 @@ def test_balance_of_rows_that_tie_or_are_masked(e, k, dtype):
     check_balance(x, k, keep)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("e,k", [(16, 4), (16, 5), (16, 16), (13, 7), (24, 5), (32, 4), (37, 8), (64, 32), (100, 9), (128, 4), (256, 8), (300, 32), (512, 31), (500, 8)])
+def test_balance_choices_among_equal_values(e, k, dtype):
+    g = torch.Generator().manual_seed(e + k)
+    for levels in (1, 2, 3, e):                        # so many different values in a row
+        x = torch.randint(0, levels, (301, e), generator=g).float()
+        x[1::7] = torch.where(torch.rand(43, e, generator=g) < 0.7, -math.inf, x[1::7])
+        x[2::7, -1] = float(torch.finfo(dtype).min)
+        x[3::7] = torch.where(torch.arange(e) >= e - k, x[3::7], torch.tensor(float(torch.finfo(dtype).min)))
+        x[4::7] *= -0.0 if levels < 3 else -1.0        # zeros of both signs are equal
+        check_balance(x.to(dtype).cuda(), k)
+
+
 def test_balance_of_any_layout():
     big = made(60, 256, torch.float32, "normal")
     check_balance(big[:, 3:19])
