@@ -80,20 +80,6 @@ template <int G, int NC> __device__ __forceinline__ float soft_max(float (&v)[NC
     return l;
 }
 
-// Descending, by Batcher's odd-even merges
-template <int N> __device__ __forceinline__ void sort_down(float (&w)[N])
-{
-#pragma unroll
-    for (int p = 1; p < N; p *= 2)
-#pragma unroll
-        for (int d = p; d >= 1; d /= 2)
-#pragma unroll
-            for (int i = 0; i < N; ++i)
-                if (i >= d % p && (i - d % p) / d % 2 == 0 && i + d < N && i / (2 * p) == (i + d) / (2 * p)) {
-                    const float hi = fmaxf(w[i], w[i + d]);
-                    w[i + d] = fminf(w[i], w[i + d]), w[i] = hi;
-                }
-}
 // Adds the k largest of a row to the bytes of `own`: equal ones by column, never one of -inf.  One after the other: the largest, the first of equal ones, then it
 // becomes -inf.
 template <typename T, int G, int NC, bool VEC> __device__ __forceinline__ void choose_in_turn(float (&u)[NC], uint32_t (&own)[NC / 4], int t, int k)
@@ -129,7 +115,10 @@ template <typename T, int G, int NC, bool VEC> __device__ __forceinline__ void c
     float w[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) w[i] = u[i];
-    sort_down(w);
+    odd_even_merges<NC>([&](int i, int j) {
+        const float hi = fmaxf(w[i], w[j]);
+        w[j] = fminf(w[i], w[j]), w[i] = hi;
+    });
     float bound = w[0];
     if (G == 1) {
 #pragma unroll

@@ -326,4 +326,16 @@ template <typename T, int TH, int NV> struct RowTrips {
     __device__ __forceinline__ const char *at(int trip) const { return first + (long long)trip * kBytes; }
 };
 
+// Batcher's odd-even merge sort of N elements: `order(i, j)`, i < j, puts the pair in order
+template <int N, typename F> __device__ __forceinline__ void odd_even_merges(F &&order)
+{
+#pragma unroll
+    for (int p = 1; p < N; p *= 2)
+#pragma unroll
+        for (int d = p; d >= 1; d /= 2)
+#pragma unroll
+            for (int i = 0; i < N; ++i)
+                if (i >= d % p && (i - d % p) / d % 2 == 0 && i + d < N && i / (2 * p) == (i + d) / (2 * p)) order(i, i + d);
+}
+
 } // namespace clb

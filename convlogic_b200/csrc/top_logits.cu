@@ -83,6 +83,20 @@ template <int TH> __device__ __forceinline__ ExpSum team_merge(ExpSum s, ExpSum 
     return lanes_merge<TH / 32>(box[threadIdx.x % (TH / 32)], c);
 }
 
+// order_key for values of 16 bits, in 16 bits, and back
+template <typename T> __device__ __forceinline__ uint32_t short_key(T v)
+{
+    const uint32_t b = raw_bits(v);
+    const float f = to_f(v);
+    return f != f ? 0xffffu : f == 0.f ? 0x8000u : b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
+}
+template <typename T> __device__ __forceinline__ float value_of_short(uint32_t key)
+{
+    float f[2];
+    two_values<T>(key == 0xffffu ? 0x7fffu : key & 0x8000u ? key & 0x7fffu : ~key & 0xffffu, f);
+    return f[0];
+}
+
 // Candidates of a team, as 32-bit numbers of their order, 0 behind the last one up to a multiple of four.  Values of 16 bits share theirs with the class (counted
 // from the segment's first), so that no two are alike; for floats, which tie seldom, the class stands beside it and is asked for only where two are alike.
 template <typename T, int CAP> struct Candidates {
@@ -93,20 +107,14 @@ template <typename T, int CAP> struct Candidates {
     __device__ __forceinline__ void put(int n, float v, int c) // c: from the segment's first class
     {
         if constexpr (kShared) {
-            const uint32_t b = raw_bits(from_f<T>(v)), k = v != v ? 0xffffu : v == 0.f ? 0x8000u : b & 0x8000u ? ~b & 0xffffu : b | 0x8000u;
-            one()[n] = k << 16 | (0xffffu - (uint32_t)c);
+            one()[n] = short_key(from_f<T>(v)) << 16 | (0xffffu - (uint32_t)c);
         } else
             one()[n] = order_key(v), cls[n] = c;
     }
     __device__ __forceinline__ float value(uint32_t o) const
     {
-        if constexpr (kShared) {
-            const uint32_t k = o >> 16, b = k == 0xffffu ? 0x7fffu : k & 0x8000u ? k & 0x7fffu : ~k & 0xffffu;
-            float f[2];
-            two_values<T>(b, f);
-            return f[0];
-        } else
-            return value_of(o);
+        if constexpr (kShared) return value_of_short<T>(o >> 16);
+        else return value_of(o);
     }
     __device__ __forceinline__ int class_at(int n) const
     {
@@ -387,7 +395,7 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
     }
 }
 
-// Rows of up to 64 classes: G lanes a row, 16 neighbouring classes each.  A class's place is the number of classes before it, counted over all pairs; with
+// Rows of up to 64 classes: G lanes a row (1 to 4), 16 neighbouring classes each.  A class's place is the number of classes before it, counted over all pairs; with
 // a warp a row 40759 rows of 3 classes took 78 us, so 7.6.
 constexpr int kFew = 16;
 template <typename T, int G>
@@ -440,6 +448,80 @@ __global__ void __launch_bounds__(kBlock) top_few_kernel(const T *__restrict__ x
         }
         l = lanes_sum<G>(l);
         if (live && t == 0) rest[r] = m / a.temperature + logf(l);
+    }
+}
+
+// Rows of up to 32 * N classes, short lists: a warp a row, N classes a lane, sorted there; the row's list is taken off the lanes' heads one by one, and what is left
+// in the lanes are the others.  An element is its order and class in one number (values of 16 bits), or the order with the class beside it.  Bound by issue:
+// 65536 rows of 100 classes, k = 10: 43 us (bf16 37), k = 100: 198 (124).
+template <typename T, int N>
+__global__ void __launch_bounds__(kBlock) top_short_kernel(const T *__restrict__ x, float *__restrict__ values, int64_t *__restrict__ indices,
+                                                           float *__restrict__ rest, TopArgs a)
+{
+    constexpr bool SHARED = sizeof(T) == 2;
+    const int lane = threadIdx.x & 31;
+    for (long long r = (long long)blockIdx.x * (kBlock / 32) + threadIdx.x / 32; r < a.rows; r += (long long)gridDim.x * (kBlock / 32)) {
+        uint32_t key[N], cls[SHARED ? 1 : N]; // 0: no class
+        T raw[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) raw[i] = i * 32 + lane < a.classes ? x[r * a.stride + i * 32 + lane] : from_f<T>(0.f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const int c = i * 32 + lane;
+            if constexpr (SHARED) key[i] = c < a.classes ? short_key(raw[i]) << 16 | (0xffffu - c) : 0;
+            else key[i] = c < a.classes ? order_key(raw[i]) : 0, cls[i] = c;
+        }
+        if constexpr (SHARED) {
+            odd_even_merges<N>([&](int i, int j) {
+                const uint32_t hi = max(key[i], key[j]);
+                key[j] = min(key[i], key[j]), key[i] = hi;
+            });
+        } else {
+            odd_even_merges<N>([&](int i, int j) {
+                const bool swap = key[j] > key[i] || (key[j] == key[i] && cls[j] < cls[i]);
+                const uint32_t k = key[i], c = cls[i];
+                key[i] = swap ? key[j] : k, cls[i] = swap ? cls[j] : c;
+                key[j] = swap ? k : key[j], cls[j] = swap ? c : cls[j];
+            });
+        }
+        auto value = [](uint32_t key) {
+            if constexpr (SHARED) return value_of_short<T>(key >> 16);
+            else return value_of(key);
+        };
+        for (int n0 = 0; n0 < a.k; n0 += 32) {
+            const int many = min(32, a.k - n0);
+            uint32_t place = 0, place_cls = 0; // of the list's next 32 the lane-th
+            for (int n = 0; n < many; ++n) {
+                const uint32_t top = __reduce_max_sync(0xffffffffu, key[0]);
+                bool taken = key[0] == top;
+                uint32_t first = 0;
+                if constexpr (!SHARED) {
+                    first = __reduce_min_sync(0xffffffffu, taken ? cls[0] : 0xffffffffu);
+                    taken = taken && cls[0] == first;
+                }
+                if (lane == n) place = top, place_cls = first;
+#pragma unroll
+                for (int i = 0; i < N; ++i) {
+                    key[i] = taken ? (i + 1 < N ? key[i + 1] : 0) : key[i];
+                    if constexpr (!SHARED)
+                        if (i + 1 < N) cls[i] = taken ? cls[i + 1] : cls[i];
+                }
+            }
+            if (lane < many) {
+                const long long at = r * a.k + n0 + lane;
+                values[at] = value(place), indices[at] = SHARED ? 0xffffu - (place & 0xffffu) : place_cls;
+            }
+        }
+        float m = -INFINITY, v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = key[i] ? value(key[i]) : -INFINITY, m = fmaxf(m, v[i]);
+        m = lanes_max<32>(m);
+        const float ref = finite_or_zero(m);
+        float l = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) l += m == INFINITY && v[i] == v[i] ? (v[i] == INFINITY ? 1.f : 0.f) : exp_of(v[i], ref, a.c);
+        l = lanes_sum<32>(l);
+        if (lane == 0) rest[r] = m / a.temperature + logf(l);
     }
 }
 
@@ -564,7 +646,21 @@ extern "C" int clb_top_logits(const void *x, int64_t row_stride, float *values, 
         u64 *const places = (u64 *)scratch;
         ExpSum *const sums = (ExpSum *)(places + (a.segments > 1 ? rows * a.segments * k : 0));
         auto blocks = [](long long n) { return (unsigned)(n < (1 << 16) ? n : (1 << 16)); }; // (then they take one row after another)
-        if (classes <= 4 * kFew) {
+        // all pairs / short / select, us, 65536 rows (fp32, bf16), k = 10: 32 classes 21 19 / 31 29 / -; 64 44 43 / 31 28 / -; 100 - / 43 37 / 88 98; 256 - / 72 56 / 94 89;
+        // 300 - / 104 88 (16 a lane) / 99 104.  A bound from groups of four classes needs more of them than the list has, or every value is a candidate: 400 classes, k = 80 and 100:
+        // select 434 295, 3705 2487, short 475 260, 562 307.
+        const bool few = classes <= 2 * kFew || (classes <= 4 * kFew && k > 20);
+        if (!few && (classes <= 256 || (classes <= 512 && 9 * k > 2 * classes))) {
+            auto go = [&](auto kernel) {
+                CLB_TRACED("top_short_kernel", st, kernel<<<blocks((rows + 7) / 8), kBlock, 0, st>>>((const T *)x, values, indices, rest, a));
+            };
+            if (classes <= 64) go(top_short_kernel<T, 2>);
+            else if (classes <= 128) go(top_short_kernel<T, 4>);
+            else if (classes <= 256) go(top_short_kernel<T, 8>);
+            else go(top_short_kernel<T, 16>);
+            return;
+        }
+        if (few) {
             const int lanes = classes <= kFew ? 1 : classes <= 2 * kFew ? 2 : 4;
             const unsigned n = blocks((rows * lanes + kBlock - 1) / kBlock);
             auto go = [&](auto kernel) { CLB_TRACED("top_few_kernel", st, kernel<<<n, kBlock, 0, st>>>((const T *)x, values, indices, rest, a)); };

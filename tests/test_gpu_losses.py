@@ -121,6 +121,17 @@ def test_top_logits_of_rows_that_tie_or_are_masked(v, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("v,k", [(33, 1), (47, 20), (64, 21), (64, 64), (65, 65), (100, 10), (100, 100), (128, 32), (128, 128), (129, 33), (200, 64), (256, 5), (256, 128),
+                                 (257, 128), (300, 66), (300, 70), (500, 128), (512, 113), (512, 128), (513, 128)])
+def test_top_logits_of_short_rows(v, k, dtype):
+    check_top(odd_rows(v, dtype, -math.inf), k)
+    check_top(made(100, v, dtype, "normal"), k, 2.5)
+    g = torch.Generator().manual_seed(v * k)
+    check_top(torch.randint(0, 4, (50, v), generator=g).to(dtype).cuda(), k, 0.5)         # equal values in all lanes
+    check_top(made(9, 2 * v + 5, dtype, "normal")[:, 3:3 + v], k)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_top_logits_of_any_layout(dtype):
     big = made(40, 1200, dtype, "normal")
     check_top(big[:, 3:1003], 9)                       # rows at a distance of their own
