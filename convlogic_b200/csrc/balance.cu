@@ -8,8 +8,8 @@
 // 64 bits: 673550 rows of 16 experts, one of them masked, 7 chosen: 1.4e-4 off with C = 0, 1.2e-5 with the plain mean, 2e-7 so.
 //
 // G lanes (1 to 32) hold a row, 16 or 32 columns each and always the same ones, so that a lane adds up its columns' probabilities and counts in registers over
-// all its rows: no atomics, the same sums every time.  Both passes are bound by HBM (or by the L2 where the logits fit it); the backward pass goes
-// through the rows from the last one on, which is what the L2 still holds.
+// all its rows: no atomics on floats, the same sums every time.  The backward pass goes through the rows from the last one on, which is what the L2 still
+// holds.  2621440 rows of 16 fp32, one choice: 41 us (4.1 TB/s) and 59 us (5.7 TB/s, reading and writing); 65536 of 128 bf16, eight choices: 25 us, issue.
 #include <algorithm>
 #include <cooperative_groups.h>
 #include <type_traits>
