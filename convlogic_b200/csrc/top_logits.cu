@@ -11,7 +11,7 @@
 // Values that tie in great numbers, more than the list holds, take a second way: bisection over all values for the k-th largest, then over the indices of those
 // that equal it.  Segments leave their k largest and the sum of their others; a block a row puts them together.
 //
-// Bound by issue: 16384 rows of 1000 bf16, k = 20: 37 us; 1024 of 128000, k = 64: 118 us for the segments (2.2 TB/s), 10 for the rows.
+// Bound by issue: 16384 rows of 1000 bf16, k = 20: 27 us; 1024 of 128000, k = 64: 97 us for the segments (2.7 TB/s), 9 for the rows.
 #include "clb_rows.cuh"
 
 using namespace clb;
@@ -46,7 +46,9 @@ template <int N> __device__ __forceinline__ uint32_t bound_of(const uint32_t (&k
         int n = 0;
 #pragma unroll
         for (int i = 0; i < N; ++i) n += key[i] >= (bound | bit);
-        if (__reduce_add_sync(0xffffffffu, n) >= k) bound |= bit;
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (n >= k) bound |= bit;
+        if ((uint32_t)(n - k) <= 4) break; // near enough (up to a quarter of k more cost a long list 10 to 30 %, to save a step or two)
     }
     return bound;
 }
@@ -165,7 +167,7 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
     constexpr int TEAMS = TH == 32 ? kBlock / TH : 1, EV = kPiece<T>, CAP = TH == 32 ? 256 : 512;
     static_assert(NV % SUB == 0 || 2 * NV == SUB, "groups of whole or half pieces");
     __shared__ Candidates<T, CAP> cand_all[TEAMS];
-    __shared__ uint32_t keys_all[TEAMS][TH * SUB];
+    __shared__ uint32_t keys_all[TEAMS][TH == 32 ? 2 : TH * SUB];
     __shared__ float extra_all[TEAMS][CAP];
     __shared__ int count_all[TEAMS], box[TH / 32 + 1];
     __shared__ uint32_t bound_all[TEAMS];
@@ -180,7 +182,7 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
         const RowPieces<T> row(x + r * a.stride, a.classes);
         const int base = seg * TH * NV;
         uint4 raw[NV];
-        row.load(raw, base + t, TH);
+        row.template load<NV, false>(raw, base + t, TH);
         // the class of value e of the thread's piece i, -1 for none
         auto class_of = [&](int i, int e) {
             const int c = row.first(base + i * TH + t) + e;
@@ -195,7 +197,7 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
         // ---- 1: the bound
         // a warp's pieces from i * TH on are not there if that is not below `used` (blocks' rows fill most of theirs)
         const int used = TH == 32 ? row.pieces - base : NV * TH;
-        uint32_t tops[NV];
+        uint32_t tops[NV], key[SUB], bound;
 #pragma unroll
         for (int i = 0; i < NV; ++i) tops[i] = i * TH < used ? piece_max_nan<T>(raw[i]) : low_word<T>();
 #pragma unroll
@@ -207,22 +209,27 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
                 for (int i = 1; i < NV / SUB; ++i) top = max_nan<T>(top, tops[s * (NV / SUB) + i]);
             } else
                 top = s & 1 ? max_nan<T>(raw[s / 2].z, raw[s / 2].w) : max_nan<T>(raw[s / 2].x, raw[s / 2].y);
-            keys_all[team][s * TH + t] = word_key<T>(top);
+            key[s] = word_key<T>(top);
         }
-        if (t == 0) count_all[team] = 0;
-        if (TH > 32)
-            for (int i = t; i < CAP / 4 + 1; i += TH) cand.four[i] = make_uint4(0, 0, 0, 0); // (what is behind the list's end)
-        team_sync<TH>();
-        if (t < 32) {
-            uint32_t key[TH * SUB / 32];
+        if constexpr (TH == 32)
+            bound = bound_of(key, a.k);
+        else {
 #pragma unroll
-            for (int i = 0; i < TH * SUB / 32; ++i) key[i] = keys_all[team][i * 32 + t];
-            const uint32_t b = bound_of(key, a.k);
-            // (fewer than k groups have a value: all values are candidates, and the first k of the masked)
-            if (t == 0) bound_all[team] = b <= kMasked ? kMasked + 1 : b;
+            for (int s = 0; s < SUB; ++s) keys_all[team][s * TH + t] = key[s];
+            if (t == 0) count_all[team] = 0;
+            for (int i = t; i < CAP / 4 + 1; i += TH) cand.four[i] = make_uint4(0, 0, 0, 0); // (what is behind the list's end)
+            __syncthreads();
+            if (t < 32) {
+                uint32_t all[TH * SUB / 32];
+#pragma unroll
+                for (int i = 0; i < TH * SUB / 32; ++i) all[i] = keys_all[team][i * 32 + t];
+                bound = bound_of(all, a.k);
+                if (t == 0) bound_all[team] = bound;
+            }
+            __syncthreads();
+            bound = bound_all[team];
         }
-        team_sync<TH>();
-        const uint32_t bound = bound_all[team];
+        if (bound <= kMasked) bound = kMasked + 1; // fewer than k groups have a value: all values are candidates, and the first k of the masked
         const bool few = bound == kMasked + 1;
         const float reach = value_of(bound);
         // ---- 2: candidates, and the sum of the others
@@ -233,76 +240,62 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
         };
         const ExpRef er = exp_ref(reach, a.c);
         float l = 0.f;
-        uint32_t hits = 0; // pieces with a candidate
+        uint32_t which_all[NV * EV / 32]; // the thread's candidates
+#pragma unroll
+        for (int i = 0; i < NV * EV / 32; ++i) which_all[i] = 0;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (i * TH >= used) continue;
-            float f[Word<T>::n];
-            Word<T>::get(tops[i], f);
-            const bool hit = !(f[0] < reach) || !(f[Word<T>::n - 1] < reach) || (few && row.first(base + i * TH + t) < own_first + a.k);
-            hits |= (uint32_t)hit << i;
             const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
                 float g[Word<T>::n];
                 Word<T>::get(w[q], g);
 #pragma unroll
-                for (int z = 0; z < Word<T>::n; ++z)
-                    if (g[z] < reach) l += ex2(fmaf(g[z], a.c, -er.R));
-            }
-        }
-        if constexpr (TH == 32) {
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-                if ((hits >> i) & 1)
-#pragma unroll
-                    for (int e = 0; e < EV; ++e) {
-                        const float v = value_at(i, e);
-                        if (!(v < reach) || few) {
-                            const int cls = class_of(i, e);
-                            if (cls >= 0 && (!(v < reach) || cls < a.k)) push(v, cls);
-                        }
-                    }
-            hits = 0;
-        }
-        while (hits) { // a warp has as many turns as its lanes have such pieces at most, one or two, not one for every piece
-            const int i = __ffs(hits) - 1;
-            hits &= hits - 1;
-            uint4 p = raw[0];
-#pragma unroll
-            for (int n = 1; n < NV; ++n) {
-                p.x = n == i ? raw[n].x : p.x, p.y = n == i ? raw[n].y : p.y;
-                p.z = n == i ? raw[n].z : p.z, p.w = n == i ? raw[n].w : p.w;
-            }
-            const uint32_t w[4] = {p.x, p.y, p.z, p.w};
-            const int first = row.first(base + i * TH + t);
-            uint32_t which = 0;
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                float f[Word<T>::n];
-                Word<T>::get(w[q], f);
-#pragma unroll
                 for (int z = 0; z < Word<T>::n; ++z) {
-                    const int e = q * Word<T>::n + z;
-                    which |= (uint32_t)!(f[z] < reach) << e;
-                    if (few && first + e >= 0 && first + e < min(a.classes, own_first + a.k)) which |= 1u << e;
+                    if (g[z] < reach) l += ex2(fmaf(g[z], a.c, -er.R));
+                    else which_all[(i * EV + q * Word<T>::n + z) / 32] |= 1u << (i * EV + q * Word<T>::n + z) % 32;
                 }
             }
-            while (which) {
-                const int e = __ffs(which) - 1;
-                which &= which - 1;
-                const int at = Word<T>::n == 1 ? e : e >> 1;
-                const uint32_t word = at == 0 ? w[0] : at == 1 ? w[1] : at == 2 ? w[2] : w[3];
-                float f[Word<T>::n];
-                Word<T>::get(word, f);
-                push(Word<T>::n == 2 && (e & 1) ? f[Word<T>::n - 1] : f[0], first + e);
+        }
+        if (few)
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < EV; ++e) {
+                    const int cls = class_of(i, e);
+                    if (cls >= own_first && cls < own_first + a.k) which_all[(i * EV + e) / 32] |= 1u << (i * EV + e) % 32;
+                }
+        int count = 0;
+#pragma unroll
+        for (int i = 0; i < NV * EV / 32; ++i) count += __popc(which_all[i]);
+        if (__any_sync(0xffffffffu, count > 0)) { // where the thread's go: behind the lanes before it, a block's warps as they come
+            int n = -count;
+#pragma unroll
+            for (int o = 1; o < 32; o *= 2) {
+                const int before = __shfl_up_sync(0xffffffffu, count, o);
+                count += (t & 31) >= o ? before : 0;
             }
+            n += count;
+            if constexpr (TH > 32) {
+                int first = 0;
+                if ((t & 31) == 31) first = atomicAdd(&count_all[team], count);
+                n += __shfl_sync(0xffffffffu, first, 31);
+            } else
+                count = __shfl_sync(0xffffffffu, count, 31);
+#pragma unroll
+            for (int i = 0; i < NV * EV / 32; ++i)
+                for (uint32_t which = which_all[i]; which; which &= which - 1, ++n) {
+                    const int at = i * 32 + __ffs(which) - 1, cls = row.first(base + at / EV * TH + t) + at % EV;
+                    // (read again: no register is named by a number that varies.  Beyond the row only where the bound is NaN and all are candidates, too many then.)
+                    if (n < CAP && cls >= 0 && cls < a.classes) cand.put(n, to_f(row.row[cls]), cls - own_first);
+                }
         }
         l = lanes_sum<32>(l * er.fix);
         if (TH > 32 && (t & 31) == 0) l_box[t >> 5] = l;
         team_sync<TH>();
-        int count = count_all[team];
-        if (TH > 32) {
+        if constexpr (TH > 32) {
+            count = count_all[team];
             l = 0.f;
 #pragma unroll
             for (int w = 0; w < TH / 32; ++w) l += l_box[w];
@@ -541,7 +534,10 @@ __global__ void __launch_bounds__(kBlock) top_merge_kernel(const u64 *__restrict
     for (long long r = blockIdx.x; r < a.rows; r += gridDim.x) {
         const u64 *p = places + r * n;
         uint32_t top = 0;
-        for (int i = t; i < n; i += kBlock) top = max(top, (uint32_t)(p[i] >> 32));
+        for (int i = 0; i < n; i += kBlock) { // (the segments' lists are in order: turned, so that a thread's are from different places of theirs, and the bound is near)
+            const int j = i + ((t + 37 * (i / kBlock)) & (kBlock - 1));
+            if (j < n) top = max(top, (uint32_t)(p[j] >> 32));
+        }
         keys[t] = top;
         if (t == 0) count_box = 0;
         __syncthreads();
@@ -675,7 +671,7 @@ extern "C" int clb_top_logits(const void *x, int64_t row_stride, float *values, 
             CLB_TRACED("top_select_kernel", st, kernel<<<blocks(n), threads, 0, st>>>((const T *)x, values, indices, rest, places, sums, a));
         };
         // Groups: more of them make a tighter bound and a longer search for it.  65536 rows of 1000 classes, 128 and 256 groups: k = 20 133 and 152 us, k = 100
-        // 582 and 362.
+        // 582 and 362 (before candidates were found by masks, which took a quarter off all of them).
         auto warps = [&](auto few, auto many) { go(k <= 32 ? few : many, (rows + 7) / 8, kBlock); };
         constexpr int SHORT = sizeof(T) == 2 ? 4 : kPieces; // half types: 1024 values of a warp, or 2048
         if (pieces <= 32 * SHORT) warps(top_select_kernel<T, 32, SHORT, 4>, top_select_kernel<T, 32, SHORT, 8>);
