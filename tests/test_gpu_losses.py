@@ -132,6 +132,20 @@ def test_top_logits_of_short_rows(v, k, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("v,k", [(600, 20), (1001, 64), (1999, 100), (5003, 64), (40001, 128)])
+def test_top_logits_of_windows(v, k, dtype):
+    """All classes but some neighbours masked, or NaN, in rows that begin anywhere."""
+    g = torch.Generator().manual_seed(v)
+    for outside in (-math.inf, math.nan):
+        wide = torch.full((24, v + 3), outside)
+        for i, w in enumerate([0, 1, k - 1, k, k + 1, 2 * k, 3 * k, 5 * k] * 3):
+            w = min(w, v)
+            at = int(torch.randint(0, v - w + 1, (1,), generator=g)) + 1
+            wide[i, at:at + w] = torch.randn(w, generator=g)
+        check_top(wide.to(dtype).cuda()[:, 1:1 + v], k, 1.5)
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 def test_top_logits_of_any_layout(dtype):
     big = made(40, 1200, dtype, "normal")
     check_top(big[:, 3:1003], 9)                       # rows at a distance of their own
