@@ -274,7 +274,8 @@ template <typename T> __device__ __forceinline__ uint32_t word_key(uint32_t w)
 // ---- (m, l) of exponents over lanes
 __device__ __forceinline__ float exp_of(float v, float m, float c) { return ex2((v - m) * c); } // of v with respect to a finite m
 // One fused multiply-add a value instead of a difference and a product: exp((v - m) / T) = exp2(v c - R) * fix with R = m c, rounded, and fix = 2^(R - m c),
-// which the rounding of R left out.  Not where m c is beyond the largest float: a maximum of the type's lowest value (every class masked with it).
+// which the rounding of R left out.  Not where that rounding is no small number (from 2^27 on it may be above 8, from 2^31 on 2^(R - m c) leaves the floats, and an
+// infinite factor makes NaN of a sum of 0): classes masked with -1e10 or the type's lowest value, or a bound far below all values.
 struct ExpRef {
     float R, fix;
     bool far;
@@ -282,7 +283,7 @@ struct ExpRef {
 __device__ __forceinline__ ExpRef exp_ref(float m, float c)
 {
     ExpRef r;
-    r.R = m * c, r.far = !(fabsf(m) < 1e38f && fabsf(r.R) < 1e38f), r.fix = ex2(-fmaf(m, c, -r.R));
+    r.R = m * c, r.far = !(fabsf(m) < 1e38f && fabsf(r.R) < 0x1p27f), r.fix = ex2(-fmaf(m, c, -r.R));
     return r;
 }
 template <int LANES> __device__ __forceinline__ float lanes_max(float v) // NaN is passed over
