@@ -26,6 +26,7 @@ struct DistillArgs {
     long long stride, rows;
     int classes, k;
     float temperature, c, scale; // c = log2(e) / T; scale: T, over the rows for a mean
+    float inv, inv_low;          // 1 / T in two parts
     int chunks, ranks_log;       // forward: how often a cluster comes back for more of a row; its blocks
 };
 
@@ -34,19 +35,28 @@ struct Entry { // one class of a list: cls < 0: does not exist
     float t, s;
 };
 
-// What a teacher's list comes to: its listed values' sum, its rest rs, the row's weight.
+// What a teacher's list comes to.  Everything is taken with respect to its largest value m: values far from zero (counts in the thousands) lose nothing but what
+// their own rounding lost.  p of value t is exp(log_p(t)).
 struct TeacherNumbers {
-    float tm, tl;   // its mass is tl * exp(tm)
-    float rest;     // probability of the rest
-    float factor;   // of the row's loss / T and gradient; 0: the row adds nothing
+    float m, ref, tl; // its mass is tl * exp(m / T + ref)
+    float d;          // log of the rest's mass, less m / T
+    float rest;       // probability of the rest
+    float factor;     // of the row's loss / T and gradient; 0: the row adds nothing
+    __device__ __forceinline__ float log_p(float t, float tt, float log_tl) const { return ((t - m) / tt - ref) - log_tl; }
 };
 __device__ __forceinline__ TeacherNumbers teacher_numbers(ExpSum teach, float rs, float w, const DistillArgs &a)
 {
     TeacherNumbers q;
-    const float tz = teach.m == -INFINITY ? -INFINITY : teach.m / a.temperature;
-    q.tm = finite_or_zero(fmaxf(tz, rs));
-    const float re = ex2((rs - q.tm) * 1.44269504f);
-    q.tl = (teach.m == -INFINITY ? teach.l : teach.l * ex2((tz - q.tm) * 1.44269504f)) + re;
+    const bool none = teach.m == -INFINITY;
+    q.m = finite_or_zero(teach.m);
+    if (fabsf(rs) < INFINITY) { // m / T by a reciprocal in two parts: rounded, it would be off by 2^-24 of itself
+        const float of_m = q.m * a.inv;
+        q.d = fabsf(of_m) < INFINITY ? fminf((rs - of_m) - fmaf(q.m, a.inv, -of_m) - q.m * a.inv_low, 3.402823466e38f) : copysignf(3.402823466e38f, -of_m);
+    } else
+        q.d = rs == -INFINITY ? rs : rs - rs;
+    q.ref = finite_or_zero(fmaxf(none ? -INFINITY : 0.f, q.d));
+    const float re = ex2((q.d - q.ref) * 1.44269504f);
+    q.tl = (none ? teach.l : teach.l * ex2(-q.ref * 1.44269504f)) + re;
     q.rest = re / q.tl;
     q.factor = q.tl != 0.f ? w * a.scale : 0.f;
     return q;
@@ -55,11 +65,11 @@ __device__ __forceinline__ TeacherNumbers teacher_numbers(ExpSum teach, float rs
 struct RowNumbers {
     float m, l, coef;  // of the unlisted scores: reference and sum; gradient = coef * exp((s - m) / T).  The list's = factor * (q - p)
     float um, ul;      // of all scores; ul = 0: there are none
-    __device__ __forceinline__ float loss(float listed, const TeacherNumbers &q, float rs, float tt) const // listed: the list's terms
+    __device__ __forceinline__ float loss(float listed, const TeacherNumbers &q, float tt) const // listed: the list's terms
     {
         if (q.rest > 0.f || q.rest != q.rest) {
             const float log_q = l == 0.f ? -INFINITY : ((m - um) / tt + logf(l)) - logf(ul);
-            listed += q.rest * (((rs - q.tm) - logf(q.tl)) - log_q);
+            listed += q.rest * (((q.d - q.ref) - logf(q.tl)) - log_q);
         }
         return listed * q.factor * tt;
     }
@@ -281,13 +291,13 @@ __global__ void __launch_bounds__(TH <= 32 ? 256 : TH, TH > 32 ? 512 / TH : NV *
         if (TH <= 32 || warp < list_warps) log_tl = logf(teach.tl), log_ul = logf(num.ul);
         auto gradient_of = [&](int n, const Entry &e) {
             if (!there || e.cls < 0) return 0.f;
-            const float lp = (e.t / tt - teach.tm) - log_tl, lq = (e.s - num.um) / tt - log_ul, p = expf(lp);
+            const float lp = teach.log_p(e.t, tt, log_tl), lq = (e.s - num.um) / tt - log_ul, p = expf(lp);
             if (p > 0.f || p != p) loss += p * (lp - lq);
             float mass = p;
             if ((twins >> (n / TH)) & 1) { // a class that is listed twice has both entries' probability
                 mass = 0.f;
                 for (int o = 0; o < a.k; ++o)
-                    if (list[o] == e.cls) mass += expf((val[o] / tt - teach.tm) - log_tl);
+                    if (list[o] == e.cls) mass += expf(teach.log_p(val[o], tt, log_tl));
             }
             return teach.factor * (expf(lq) - mass);
         };
@@ -312,7 +322,7 @@ __global__ void __launch_bounds__(TH <= 32 ? 256 : TH, TH > 32 ? 512 / TH : NV *
                 loss = 0.f;
                 for (int i = 0; i < list_warps; ++i) loss += loss_part[i];
             }
-            row_loss[r] = there ? num.loss(loss, teach, rs, tt) : 0.f;
+            row_loss[r] = there ? num.loss(loss, teach, tt) : 0.f;
             stats[2 * r] = m, stats[2 * r + 1] = coef;
         }
         team_sync(); // the tables are used again
@@ -432,13 +442,13 @@ __global__ void __launch_bounds__(TH, 1024 / TH)
             for (int i = 0; i < EACH; ++i) {
                 g[i] = 0.f;
                 if (there && cls[i] >= 0) {
-                    const float lp = (tv[i] / tt - q.tm) - log_tl, lq = (sv[i] - n.um) / tt - log_ul, p = expf(lp);
+                    const float lp = q.log_p(tv[i], tt, log_tl), lq = (sv[i] - n.um) / tt - log_ul, p = expf(lp);
                     if (p > 0.f || p != p) loss += p * (lp - lq);
                     float mass = p;
                     if (dup) { // a class that is listed twice has both entries' probability
                         mass = 0.f;
                         for (int o = 0; o < a.k; ++o)
-                            if (list[o] == cls[i]) mass += expf((values[r * a.k + o] / tt - q.tm) - log_tl);
+                            if (list[o] == cls[i]) mass += expf(q.log_p(values[r * a.k + o], tt, log_tl));
                     }
                     g[i] = q.factor * (expf(lq) - mass);
                 }
@@ -446,7 +456,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH)
             }
             loss = lanes_sum<32>(loss);
             if (lane == 0) {
-                row_loss[r] = there ? n.loss(loss, q, rs, tt) : 0.f;
+                row_loss[r] = there ? n.loss(loss, q, tt) : 0.f;
                 stats[2 * r] = n.m, stats[2 * r + 1] = n.coef;
             }
             next_dup = mark(r + gridDim.x, tables + (odd ^ 1) * words);
@@ -639,8 +649,9 @@ bool sizes_ok(int64_t rows, int64_t classes, int64_t row_stride, int k, double t
 }
 DistillArgs make_args(int64_t rows, int64_t classes, int64_t row_stride, int k, double temperature, int reduction)
 {
+    const float inv = (float)(1.0 / temperature);
     return {row_stride, rows, (int)classes, k, (float)temperature, (float)(1.4426950408889634 / temperature),
-            (float)(reduction == CLB_REDUCE_MEAN && rows > 0 ? temperature / (double)rows : temperature)};
+            (float)(reduction == CLB_REDUCE_MEAN && rows > 0 ? temperature / (double)rows : temperature), inv, (float)(1.0 / temperature - inv)};
 }
 
 constexpr long long kMostBlocks = 1 << 16; // then they take one row after another

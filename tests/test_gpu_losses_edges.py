@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import loss_oracle
-from tests.test_gpu_losses import DTYPES, IDS, check_distill, check_top, lists_for, made
+from tests.test_gpu_losses import DTYPES, IDS, check_distill, check_grad, check_loss, check_top, lists_for, made
 
 pytestmark = pytest.mark.gpu
 
@@ -65,3 +65,45 @@ def test_distillation_of_classes_masked_with_a_number(n, v, mask, dtype):
         top = (values, indices, rest if with_rest else None)
         check_distill(x, top, 1.5, None, "none", up)
         check_distill(x, top, 1.5, None, "sum", None)
+
+
+# ------------------------------------------------------------------------------------------------ lists far from zero
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("shift", [0.0, 3e3, -1e4, 1e6])
+@pytest.mark.parametrize("n,v", [(7, 20), (7, 1000), (7, 5000), (3, 70001), (66, 2100), (66, 20000)])
+def test_lists_far_from_zero(n, v, shift, dtype):
+    """A teacher's counts in the thousands: probabilities are those of the differences, and of the rest's distance from them, as the lists hold both in 32 bits."""
+    x = made(n, v, dtype, "normal")
+    values, indices, rest = lists_for(x, 12, 1.7)
+    indices[1, 3] = indices[1, 0]                      # a class listed twice adds up both
+    values = values + shift
+    rest = (rest.double() + shift / 1.7).float()
+    up = torch.rand(n, generator=torch.Generator().manual_seed(2)).cuda() + 0.5
+    for with_rest in (True, False):
+        check_distill(x, (values, indices, rest if with_rest else None), 1.7, None, "none", up)
+    check_distill(x, (values, indices, rest), 1.7, None, "sum")
+
+
+@pytest.mark.parametrize("temperature", [0.25, 0.5, 1.0, 3.0])
+@pytest.mark.parametrize("n,v", [(6, 40), (6, 3000), (3, 70001), (66, 2100)])
+def test_lists_of_the_lowest_and_the_largest_values(n, v, temperature):
+    """Equal values are equal probabilities, whatever they are: the lists of zeros give the loss.  A rest beside the lowest is everything, beside the largest nothing."""
+    import convlogic_b200 as cb
+
+    x = made(n, v, torch.float32, "normal")
+    _, indices, _ = lists_for(x, 4, 1.0)
+    zeros, rest = torch.zeros(n, 4, device="cuda"), torch.full((n,), 2.0, device="cuda")
+
+    def both(values, rest):
+        leaf = x.clone().requires_grad_(True)
+        loss = cb.distillation_loss(leaf, (values, indices, rest), temperature, reduction="none")
+        return loss.detach(), torch.autograd.grad(loss, leaf, torch.ones_like(loss))[0]
+
+    alike = both(zeros, None)
+    for value in (torch.finfo(torch.float32).min, torch.finfo(torch.float32).max, -1e30, 1e30):
+        values = torch.full_like(zeros, value)
+        assert all(torch.equal(a, b) for a, b in zip(both(values, None), alike)), value
+        loss, grad = both(values, rest)
+        want = loss_oracle.distillation(x, zeros - (1e30 if value < 0 else 0.0), indices, rest if value < 0 else rest - 1e30, None, temperature, "none")
+        check_loss(loss, want["loss"], want["loss_scale"])
+        check_grad(grad, want["grad"], want["grad_scale"], x.dtype)
