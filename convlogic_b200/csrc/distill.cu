@@ -61,16 +61,27 @@ __device__ __forceinline__ TeacherNumbers teacher_numbers(ExpSum teach, float rs
     q.factor = q.tl != 0.f ? w * a.scale : 0.f;
     return q;
 }
+// A class's share of the loss, p log(p / q) - p + q with delta = log(p / q): what is added to p log(p / q) comes to nothing over all classes, but for what the logarithms
+// of the sums are off, and takes the cancellation out: no share is below 0, and an error of a logarithm counts with p - q, not with p.  (A list that holds little of
+// the mass, or a student near its teacher: losses of 1e-4 were 1e-2 off.)
+__device__ __forceinline__ float share_of(float p, float delta, float q)
+{
+    if (p == 0.f) return q;
+    if (!(fabsf(delta) < 0.5f)) return p * (delta - 1.f) + q;
+    const float d = delta; // exp(-d) - 1 + d, Taylor's
+    float f = fmaf(d, -1.f / 362880, 1.f / 40320);
+    f = fmaf(d, f, -1.f / 5040), f = fmaf(d, f, 1.f / 720), f = fmaf(d, f, -1.f / 120), f = fmaf(d, f, 1.f / 24), f = fmaf(d, f, -1.f / 6), f = fmaf(d, f, 0.5f);
+    return p * (d * d) * f;
+}
 // What a row's sums come to: unlisted scores `rest`, distinct listed ones `list`.
 struct RowNumbers {
     float m, l, coef;  // of the unlisted scores: reference and sum; gradient = coef * exp((s - m) / T).  The list's = factor * (q - p)
     float um, ul;      // of all scores; ul = 0: there are none
+    float qr;          // probability of the unlisted ones
     __device__ __forceinline__ float loss(float listed, const TeacherNumbers &q, float tt) const // listed: the list's terms
     {
-        if (q.rest > 0.f || q.rest != q.rest) {
-            const float log_q = l == 0.f ? -INFINITY : ((m - um) / tt + logf(l)) - logf(ul);
-            listed += q.rest * (((q.d - q.ref) - logf(q.tl)) - log_q);
-        }
+        const float log_qr = l == 0.f ? -INFINITY : ((m - um) / tt + logf(l)) - logf(ul);
+        listed += share_of(q.rest, ((q.d - q.ref) - logf(q.tl)) - log_qr, qr);
         return listed * q.factor * tt;
     }
 };
@@ -80,7 +91,8 @@ __device__ __forceinline__ RowNumbers row_numbers(ExpSum rest, ExpSum list, cons
     n.m = finite_or_zero(rest.m), n.um = finite_or_zero(fmaxf(rest.m, list.m)), n.l = rest.l;
     const float of_rest = rest.l == 0.f ? 0.f : rest.l * exp_of(n.m, n.um, a.c);
     n.ul = of_rest + (list.l == 0.f ? 0.f : list.l * exp_of(finite_or_zero(list.m), n.um, a.c));
-    n.coef = q.factor == 0.f || rest.l == 0.f ? 0.f : q.factor * __fdividef(__fdividef(of_rest, n.ul) - q.rest, rest.l);
+    n.qr = __fdividef(of_rest, n.ul);
+    n.coef = q.factor == 0.f || rest.l == 0.f ? 0.f : q.factor * __fdividef(n.qr - q.rest, rest.l);
     return n;
 }
 
@@ -291,15 +303,16 @@ __global__ void __launch_bounds__(TH <= 32 ? 256 : TH, TH > 32 ? 512 / TH : NV *
         if (TH <= 32 || warp < list_warps) log_tl = logf(teach.tl), log_ul = logf(num.ul);
         auto gradient_of = [&](int n, const Entry &e) {
             if (!there || e.cls < 0) return 0.f;
-            const float lp = teach.log_p(e.t, tt, log_tl), lq = (e.s - num.um) / tt - log_ul, p = expf(lp);
-            if (p > 0.f || p != p) loss += p * (lp - lq);
+            const float lp = teach.log_p(e.t, tt, log_tl), lq = (e.s - num.um) / tt - log_ul, p = expf(lp), q = expf(lq);
             float mass = p;
             if ((twins >> (n / TH)) & 1) { // a class that is listed twice has both entries' probability
                 mass = 0.f;
                 for (int o = 0; o < a.k; ++o)
                     if (list[o] == e.cls) mass += expf(teach.log_p(val[o], tt, log_tl));
-            }
-            return teach.factor * (expf(lq) - mass);
+                loss += (p == 0.f ? 0.f : p * (lp - lq - 1.f)) + ((firsts >> (n / TH)) & 1 ? q : 0.f);
+            } else
+                loss += share_of(p, lp - lq, q);
+            return teach.factor * (q - mass);
         };
         if (TH > 32) {
             if (warp < list_warps) {
@@ -442,15 +455,17 @@ __global__ void __launch_bounds__(TH, 1024 / TH)
             for (int i = 0; i < EACH; ++i) {
                 g[i] = 0.f;
                 if (there && cls[i] >= 0) {
-                    const float lp = q.log_p(tv[i], tt, log_tl), lq = (sv[i] - n.um) / tt - log_ul, p = expf(lp);
-                    if (p > 0.f || p != p) loss += p * (lp - lq);
+                    const float lp = q.log_p(tv[i], tt, log_tl), lq = (sv[i] - n.um) / tt - log_ul, p = expf(lp), qk = expf(lq);
                     float mass = p;
                     if (dup) { // a class that is listed twice has both entries' probability
                         mass = 0.f;
+                        bool first = true;
                         for (int o = 0; o < a.k; ++o)
-                            if (list[o] == cls[i]) mass += expf(q.log_p(values[r * a.k + o], tt, log_tl));
-                    }
-                    g[i] = q.factor * (expf(lq) - mass);
+                            if (list[o] == cls[i]) mass += expf(q.log_p(values[r * a.k + o], tt, log_tl)), first = first && o >= lane + 32 * i;
+                        loss += (p == 0.f ? 0.f : p * (lp - lq - 1.f)) + (first ? qk : 0.f);
+                    } else
+                        loss += share_of(p, lp - lq, qk);
+                    g[i] = q.factor * (qk - mass);
                 }
                 if (lane + 32 * i < a.k) listed[r * a.k + lane + 32 * i] = g[i];
             }

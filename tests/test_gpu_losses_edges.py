@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import loss_oracle
-from tests.test_gpu_losses import DTYPES, IDS, check_distill, check_grad, check_loss, check_top, lists_for, made
+from tests.test_gpu_losses import DTYPES, EPS, IDS, check_distill, check_grad, check_loss, check_top, lists_for, made
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,25 @@ def test_lists_of_the_lowest_and_the_largest_values(n, v, temperature):
         want = loss_oracle.distillation(x, zeros - (1e30 if value < 0 else 0.0), indices, rest if value < 0 else rest - 1e30, None, temperature, "none")
         check_loss(loss, want["loss"], want["loss_scale"])
         check_grad(grad, want["grad"], want["grad_scale"], x.dtype)
+
+
+# ------------------------------------------------------------------------------------------------ losses near zero
+@pytest.mark.parametrize("n,v,k", [(8, 6, 6), (8, 12, 3), (8, 100, 20), (8, 1000, 1), (8, 1000, 64), (8, 5000, 16), (3, 70001, 1), (3, 140003, 32), (66, 2100, 40), (66, 20000, 1), (66, 40001, 100)])
+def test_losses_near_zero(n, v, k):
+    """A student near its teacher, and lists that hold little of the mass.  A loss is sum p f(delta) with f(d) = d - 1 + exp(-d) over all classes, delta = log p - log q: an error e of a
+    delta costs |p - q| e + p e^2 / 2.  Deltas are differences of logarithms of sums, 2 EPS = 1e-4 off at most; sum |p - q| is what the gradient's magnitudes add up to,
+    by T; the shares themselves are products, 16 * 2^-24."""
+    import convlogic_b200 as cb
+
+    t = 4.0
+    g = torch.Generator().manual_seed(v + k)
+    for noise in (3.0, 0.1, 0.01):
+        x = torch.randn(n, v, generator=g)
+        teacher = x + noise * torch.randn(n, v, generator=g)
+        values, indices, rest = loss_oracle.top_logits(teacher, k, t)
+        top = (values.float().cuda(), indices.cuda(), rest.float().cuda())
+        loss = cb.distillation_loss(x.cuda(), top, t, reduction="none").cpu().double()
+        want = loss_oracle.distillation(x, *(s.cpu() for s in top), None, t, "none")
+        off = t * want["grad"].abs().sum(1)
+        bound = 2 * EPS * off + 2 * t * t * (2 * EPS) ** 2 + 16 * 2.0 ** -24 * want["loss"]
+        assert ((loss - want["loss"]).abs() <= bound).all(), (noise, loss, want["loss"], bound)
