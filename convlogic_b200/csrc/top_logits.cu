@@ -12,6 +12,8 @@
 // that equal it.  Segments leave their k largest and the sum of their others; a block a row puts them together.
 //
 // Bound by issue: 16384 rows of 1000 bf16, k = 20: 27 us; 1024 of 128000, k = 64: 97 us for the segments (2.7 TB/s), 9 for the rows.
+#include <algorithm>
+
 #include "clb_rows.cuh"
 
 using namespace clb;
@@ -165,7 +167,7 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
                                                                float *__restrict__ rest, u64 *__restrict__ places, ExpSum *__restrict__ sums, TopArgs a)
 {
     constexpr int TEAMS = TH == 32 ? kBlock / TH : 1, EV = kPiece<T>, CAP = TH == 32 ? 256 : 512;
-    static_assert(NV % SUB == 0 || 2 * NV == SUB, "groups of whole or half pieces");
+    static_assert(NV % SUB == 0 || 2 * NV == SUB || 4 * NV == SUB, "groups of whole pieces, of half a piece, or of one word");
     __shared__ Candidates<T, CAP> cand_all[TEAMS];
     __shared__ uint32_t keys_all[TEAMS][TH == 32 ? 2 : TH * SUB];
     __shared__ float extra_all[TEAMS][CAP];
@@ -207,8 +209,10 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
                 top = tops[s * (NV / SUB)];
 #pragma unroll
                 for (int i = 1; i < NV / SUB; ++i) top = max_nan<T>(top, tops[s * (NV / SUB) + i]);
-            } else
+            } else if constexpr (2 * NV == SUB)
                 top = s & 1 ? max_nan<T>(raw[s / 2].z, raw[s / 2].w) : max_nan<T>(raw[s / 2].x, raw[s / 2].y);
+            else
+                top = (&raw[s / 4].x)[s % 4];
             key[s] = word_key<T>(top);
         }
         if constexpr (TH == 32)
@@ -670,14 +674,27 @@ extern "C" int clb_top_logits(const void *x, int64_t row_stride, float *values, 
         auto go = [&](auto kernel, long long n, int threads) {
             CLB_TRACED("top_select_kernel", st, kernel<<<blocks(n), threads, 0, st>>>((const T *)x, values, indices, rest, places, sums, a));
         };
-        // Groups: more of them make a tighter bound and a longer search for it.  65536 rows of 1000 classes, 128 and 256 groups: k = 20 133 and 152 us, k = 100
-        // 582 and 362 (before candidates were found by masks, which took a quarter off all of them).
-        auto warps = [&](auto few, auto many) { go(k <= 32 ? few : many, (rows + 7) / 8, kBlock); };
+        // Groups: more of them make a tighter bound and a longer search for it.  Where few more than k of them have values, the bound lets through more values than the
+        // list holds and the row takes the second way.  Plain / twice as many groups, us, 33 million values, by groups / k: fp32 257 classes k = 32 (1.0) 423 / 136, k = 16
+        // (2.1) 93 / 101; 513 k = 128 (1.0) 4185 / 518, k = 64 (2.0) 229 / 239; 640 k = 90 (1.8) 294 / 260; bf16 1025 k = 128 (1.0) 2987 / 228, 2049 k = 90 (1.4) 132 / 111,
+        // k = 64 (2.0) 90 / 101.  Lists of 90 are even from 2.1 on, longer ones always shorter by the tighter bound: fp32 1000 k = 110 (2.3) 239 / 199.
+        auto enough = [&](long long groups) { return 5 * groups >= 9 * k; };
+        auto groups = [&](int threads, int pieces_each, int subs) { // that have values
+            long long n = 0;
+            for (int s = 0, first = 0; s < subs && subs < pieces_each; ++s, first += pieces_each / subs * threads) n += std::max(0ll, std::min<long long>(threads, pieces - first));
+            return subs < pieces_each ? n : pieces * (subs / pieces_each);
+        };
+        auto warps = [&](auto few, auto many, auto most, int pieces_each) {
+            const long long n = (rows + 7) / 8;
+            if (k <= 32 && enough(groups(32, pieces_each, 4))) go(few, n, kBlock);
+            else if (k <= 96 && enough(groups(32, pieces_each, 8))) go(many, n, kBlock);
+            else go(most, n, kBlock);
+        };
         constexpr int SHORT = sizeof(T) == 2 ? 4 : kPieces; // half types: 1024 values of a warp, or 2048
-        if (pieces <= 32 * SHORT) warps(top_select_kernel<T, 32, SHORT, 4>, top_select_kernel<T, 32, SHORT, 8>);
-        else if (pieces <= 32 * kPieces) warps(top_select_kernel<T, 32, kPieces, 4>, top_select_kernel<T, 32, kPieces, 8>);
-        else if (pieces <= 64 * kPieces) go(top_select_kernel<T, 64, kPieces, 4>, rows, 64);
-        else if (pieces <= 128 * kPieces) go(top_select_kernel<T, 128, kPieces, 2>, rows, 128);
+        if (pieces <= 32 * SHORT) warps(top_select_kernel<T, 32, SHORT, 4>, top_select_kernel<T, 32, SHORT, 8>, top_select_kernel<T, 32, SHORT, 16>, SHORT);
+        else if (pieces <= 32 * kPieces) warps(top_select_kernel<T, 32, kPieces, 4>, top_select_kernel<T, 32, kPieces, 8>, top_select_kernel<T, 32, kPieces, 16>, kPieces);
+        else if (pieces <= 64 * kPieces) go(k <= 96 && enough(groups(64, kPieces, 4)) ? top_select_kernel<T, 64, kPieces, 4> : top_select_kernel<T, 64, kPieces, 8>, rows, 64);
+        else if (pieces <= 128 * kPieces) go(k <= 96 && enough(groups(128, kPieces, 2)) ? top_select_kernel<T, 128, kPieces, 2> : top_select_kernel<T, 128, kPieces, 4>, rows, 128);
         else go(top_select_kernel<T, kBlock, kPieces, 1>, rows * a.segments, kBlock);
         if (a.segments > 1) {
             CLB_TRACED("top_merge_kernel", st, top_merge_kernel<<<blocks(rows), kBlock, 0, st>>>(places, sums, values, indices, rest, a));

@@ -129,3 +129,33 @@ def test_losses_near_zero(n, v, k):
         off = t * want["grad"].abs().sum(1)
         bound = 2 * EPS * off + 2 * t * t * (2 * EPS) ** 2 + 16 * 2.0 ** -24 * want["loss"]
         assert ((loss - want["loss"]).abs() <= bound).all(), (noise, loss, want["loss"], bound)
+
+
+# ------------------------------------------------------------------------------------------------ sizes just past a kernel's
+def _time(call, n=5):
+    """The shortest of five times of a call, each the mean of n."""
+    call()
+    times = []
+    for _ in range(5):
+        a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+        a.record()
+        for _ in range(n):
+            call()
+        b.record()
+        torch.cuda.synchronize()
+        times.append(a.elapsed_time(b) / n)
+    return min(times)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("v,k,more", [(257, 32, 420), (257, 57, 420), (513, 113, 640), (513, 128, 640), (540, 128, 640), (1025, 116, 1700), (1025, 128, 1700), (1100, 128, 1700), (2049, 128, 3500),
+                                      (2049, 110, 3500), (4097, 128, 6500)])
+def test_top_logits_just_past_a_size(v, k, more, dtype):
+    """A row that is a little longer than a kernel's shorter rows has few groups of neighbours, and a list almost as long: right, and no slower than the values that it has not.
+    (Where a row's values all are candidates it takes 6 to 30 times as long.)"""
+    import convlogic_b200 as cb
+
+    check_top(made(40, v, dtype, "normal"), k)
+    check_top(made(40, v + 9, dtype, "wide")[:, 3:3 + v], k, 2.0)
+    short, long = (torch.randn(8192, w, device="cuda").to(dtype) for w in (v, more))
+    assert _time(lambda: cb.top_logits(short, k)) < 2.0 * _time(lambda: cb.top_logits(long, k))
