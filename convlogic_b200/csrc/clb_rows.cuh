@@ -133,15 +133,15 @@ template <typename T> struct RowPieces {
             }
         return make_uint4(w[0], w[1], w[2], w[3]);
     }
-    // pieces j, j + step, ...: the whole ones are asked for before anything waits.  LAST: not read again
-    template <int NV, bool LAST = true> __device__ __forceinline__ void load(uint4 (&q)[NV], int j, int step) const
+    // pieces j, j + step, ...: the whole ones are asked for before anything waits.  LAST: not read again.  BOUND: none from `end` on (of the same step as those)
+    template <int NV, bool LAST = true, bool BOUND = false> __device__ __forceinline__ void load(uint4 (&q)[NV], int j, int step, int end = 0) const
     {
         const T *const from = row + first(j);
         auto get = [&](int i) {
             const uint4 *p = reinterpret_cast<const uint4 *>(from + (long long)i * step * kPiece<T>);
             return LAST ? __ldcs(p) : __ldg(p);
         };
-        if (inside<NV>(j, step)) {
+        if (inside<NV>(j, step) && (!BOUND || j + (NV - 1) * step < end)) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) q[i] = get(i);
             return;
@@ -149,11 +149,11 @@ template <typename T> struct RowPieces {
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             q[i] = make_uint4(low_word<T>(), low_word<T>(), low_word<T>(), low_word<T>());
-            if (whole(j + i * step)) q[i] = get(i);
+            if (whole(j + i * step) && (!BOUND || j + i * step < end)) q[i] = get(i);
         }
         if (j == 0 && !whole(0)) q[0] = edge(0); // (a first piece is some thread's first)
         const int last = pieces - 1, i = last - j;
-        if (last > 0 && i >= 0 && i < NV * step && i % step == 0 && !whole(last)) {
+        if (last > 0 && i >= 0 && i < NV * step && i % step == 0 && (!BOUND || last < end) && !whole(last)) {
             const uint4 e = edge(last);
 #pragma unroll
             for (int n = 0; n < NV; ++n) {

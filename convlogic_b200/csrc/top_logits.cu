@@ -2,8 +2,8 @@
 //
 // A row's classes are ordered by value, ties by index; the first k are the list, and rest = log sum over the others of exp(x / T).
 //
-// One read of the logits.  Short rows are sorted whole: by counting pairs or in a warp's lanes.  Else a team of threads (a warp for rows of up to 1024 fp32 or 2048 half values; a block for longer ones, or for a segment of 32 KB, so
-// that one row, too, fills part of the GPU) holds its values in registers:
+// One read of the logits.  Short rows are sorted whole: by counting pairs or in a warp's lanes.  Else a team of threads (a warp for rows of up to 1024 fp32 or 2048 half values; a block for longer ones, or for a segment of at
+// most 32 KB, so that one row, too, fills part of the GPU) holds its values in registers:
 //   1. The k-th largest of the threads' own maxima, rounded down to 16 bits of its order, is a bound that at least k values reach, and few more: with 256 maxima
 //      of 64 values about 75 for k = 64.  One warp finds it by bisection.
 //   2. The values that reach the bound go to a list in shared memory; the others are added up as exponentials with respect to the bound.
@@ -58,6 +58,7 @@ template <int N> __device__ __forceinline__ uint32_t bound_of(const uint32_t (&k
 struct TopArgs {
     long long stride, rows;
     int classes, k, segments;
+    int slots, longer; // pieces of each thread in a segment, one more in the first `longer` segments
     float temperature, c; // c = log2(e) / T
 };
 
@@ -182,13 +183,15 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
         const long long r = a.segments == 1 ? item : item / a.segments;
         const int seg = a.segments == 1 ? 0 : (int)(item - r * a.segments);
         const RowPieces<T> row(x + r * a.stride, a.classes);
-        const int base = seg * TH * NV;
+        // (segments of like lengths: what a last one of a few classes lists is all candidates, which takes the second way: 1973 rows of 17000 bf16, k = 100: 1091 us)
+        const int slots = TH == kBlock ? a.slots + (seg < a.longer) : NV;
+        const int base = TH == kBlock ? (seg * a.slots + min(seg, a.longer)) * TH : 0;
         uint4 raw[NV];
-        row.template load<NV, false>(raw, base + t, TH);
+        row.template load<NV, false, TH == kBlock>(raw, base + t, TH, base + slots * TH);
         // the class of value e of the thread's piece i, -1 for none
         auto class_of = [&](int i, int e) {
             const int c = row.first(base + i * TH + t) + e;
-            return c >= 0 && c < a.classes ? c : -1;
+            return c >= 0 && c < a.classes && i < slots ? c : -1;
         };
         auto value_at = [&](int i, int e) {
             const uint32_t w = (&raw[i].x)[sizeof(T) == 4 ? e & 3 : e >> 1];
@@ -197,8 +200,8 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
             return f[Word<T>::n == 1 ? 0 : e & 1];
         };
         // ---- 1: the bound
-        // a warp's pieces from i * TH on are not there if that is not below `used` (blocks' rows fill most of theirs)
-        const int used = TH == 32 ? row.pieces - base : NV * TH;
+        // pieces from i * TH on are not there if that is not below `used` (rows of blocks of 64 and 128 threads fill most of theirs)
+        const int used = TH == 32 ? row.pieces : slots * TH;
         uint32_t tops[NV], key[SUB], bound;
 #pragma unroll
         for (int i = 0; i < NV; ++i) tops[i] = i * TH < used ? piece_max_nan<T>(raw[i]) : low_word<T>();
@@ -358,8 +361,6 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
             } else
                 extra_all[team][rank - a.k] = v;
         });
-        if (a.segments > 1)
-            for (int n = count + t; n < a.k; n += TH) places[at + n] = 0; // a last segment of few classes
         team_sync<TH>();
         auto finish = [&](ExpSum others) {
             if (a.segments == 1) rest[r] = others.m / a.temperature + logf(others.l);
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(TH == 32 ? kBlock : TH, TH == 32 ? 4 : 4 * kBl
         };
         if (overflow || er.far || !(reach < INFINITY) || (!(l > 1e-20f) && count <= a.k)) {
             // the bound is no reference for the others (they are far below it), or they are not all counted: once more, with respect to their own largest
-            const u64 kth = count >= a.k ? place_of(kth_box[0], kth_box[1]) : 0;
+            const u64 kth = place_of(kth_box[0], kth_box[1]);
             ExpSum others{-INFINITY, 0.f};
             bool inf = false;
             for_each([&](float v, int cls) {
@@ -553,7 +554,7 @@ __global__ void __launch_bounds__(kBlock) top_merge_kernel(const u64 *__restrict
             if (t == 0) bound_box = b;
         }
         __syncthreads();
-        const uint32_t bound = max(bound_box, 1u); // (0: no value)
+        const uint32_t bound = bound_box;
         for (int i = t; i < n; i += kBlock)
             if ((uint32_t)(p[i] >> 32) >= bound) {
                 const int c = atomicAdd(&count_box, 1);
@@ -596,7 +597,7 @@ __global__ void __launch_bounds__(kBlock) top_merge_kernel(const u64 *__restrict
             else others = merge(others, s, a.c);
         };
         for (int i = t; i < n; i += kBlock)
-            if (p[i] && p[i] < kth) add(single(value_of((uint32_t)(p[i] >> 32))));
+            if (p[i] < kth) add(single(value_of((uint32_t)(p[i] >> 32))));
         for (int i = t; i < a.segments; i += kBlock) add(sums[r * a.segments + i]);
         others = team_merge<kBlock>(others, sum_box, a.c);
         if (team_count<kBlock>(inf, box) && others.l == others.l) others = ExpSum{INFINITY, 1.f};
@@ -613,10 +614,8 @@ template <typename T> long long most_pieces(const void *x, int64_t stride, int64
     const int phase = !any && (rows == 1 || stride % kPiece<T> == 0) ? (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) : kPiece<T> - 1;
     return (classes + phase + kPiece<T> - 1) / kPiece<T>;
 }
-template <typename T> int segments_of(long long pieces)
-{
-    return (int)((pieces + kBlock * kPieces - 1) / (kBlock * kPieces));
-}
+int slots_of(long long pieces) { return (int)((pieces + kBlock - 1) / kBlock); } // pieces of each thread of a block
+int segments_of(long long pieces) { return (slots_of(pieces) + kPieces - 1) / kPieces; }
 
 } // namespace
 
@@ -624,7 +623,7 @@ extern "C" size_t clb_top_logits_scratch_bytes(int64_t rows, int64_t classes, in
 {
     if (rows <= 0 || classes <= 0 || k <= 0 || classes > CLB_CLASSES_MAX) return 0;
     int segments = 0;
-    with_score_type(dtype, [&](auto t) { segments = segments_of<decltype(t)>(most_pieces<decltype(t)>(nullptr, 1, rows, classes, true)); });
+    with_score_type(dtype, [&](auto t) { segments = segments_of(most_pieces<decltype(t)>(nullptr, 1, rows, classes, true)); });
     return segments > 1 ? (size_t)rows * segments * (8 * (size_t)k + sizeof(ExpSum)) : 0;
 }
 
@@ -644,7 +643,8 @@ extern "C" int clb_top_logits(const void *x, int64_t row_stride, float *values, 
     with_score_type(dtype, [&](auto v) {
         using T = decltype(v);
         const long long pieces = most_pieces<T>(x, row_stride, rows, classes);
-        TopArgs a{row_stride, rows, (int)classes, k, segments_of<T>(pieces), (float)temperature, (float)(1.4426950408889634 / temperature)};
+        const int segments = segments_of(pieces);
+        TopArgs a{row_stride, rows, (int)classes, k, segments, slots_of(pieces) / segments, slots_of(pieces) % segments, (float)temperature, (float)(1.4426950408889634 / temperature)};
         u64 *const places = (u64 *)scratch;
         ExpSum *const sums = (ExpSum *)(places + (a.segments > 1 ? rows * a.segments * k : 0));
         auto blocks = [](long long n) { return (unsigned)(n < (1 << 16) ? n : (1 << 16)); }; // (then they take one row after another)
