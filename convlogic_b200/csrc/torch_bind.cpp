@@ -1567,6 +1567,7 @@ PYBIND11_MODULE(_clb_torch, m)
     m.def("balance_loss", &balance_loss);
     m.def("balance_fwd", &balance_fwd_py);
     m.def("balance_bwd", &balance_bwd_py);
+    m.def("once", [](const Tensor &g, const Tensor &x) { return once(g, x)[0]; });
     m.def("transpose2d", &transpose2d);
     m.def("adam_step", &adam_step);
     m.def("count_sinks", [](int64_t change) { g_sinks += change; });

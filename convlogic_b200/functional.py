@@ -302,7 +302,7 @@ class DistillationFunction(Function):
     @staticmethod
     def backward(ctx, gloss):
         scores, indices, stats, listed = ctx.saved_tensors
-        return (ops.distill_bwd(gloss.float(), scores, indices, stats, listed, ctx.temperature),) + (None,) * 6
+        return (native().once(ops.distill_bwd(gloss.float(), scores, indices, stats, listed, ctx.temperature), scores),) + (None,) * 6
 
 
 class BalanceFunction(Function):
@@ -318,7 +318,7 @@ class BalanceFunction(Function):
     @staticmethod
     def backward(ctx, gloss, unused):
         logits, share, keep = ctx.saved_tensors
-        return ops.balance_bwd(gloss.float(), logits, share, keep), None, None
+        return native().once(ops.balance_bwd(gloss.float(), logits, share, keep), logits), None, None
 
 
 class FeatureMajorFunction(Function):

@@ -1,0 +1,36 @@
+"""The loss terms where something else follows the call: torch.jit.trace, a second derivative, a gradient bucket, another stream."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+
+def _scores(n=12, v=40, seed=0):
+    return (torch.randn(n, v, generator=torch.Generator().manual_seed(seed)) * 3).cuda()
+
+
+def _terms(top):
+    """Each loss as a call of its own, as the trace of it, and as its Function."""
+    import convlogic_b200 as cb
+    from convlogic_b200 import functional
+
+    plain = {"distillation": lambda s: cb.distillation_loss(s, top), "balance": lambda s: cb.balance_loss(s, 2)[0]}
+    traced = {name + " traced": torch.jit.trace(f, (_scores(),), check_trace=False) for name, f in plain.items()}
+    apply = {"distillation applied": lambda s: functional.DistillationFunction.apply(s, *top[:3], None, 1.0, "mean"),
+             "balance applied": lambda s: functional.BalanceFunction.apply(s, 2, None)[0]}
+    return {**plain, **traced, **apply}
+
+
+def test_a_second_derivative_is_refused_wherever_the_first_came_from():
+    """Beside another term that keeps the sum differentiable, too: nothing is left out without a word."""
+    import convlogic_b200 as cb
+
+    top = cb.top_logits(_scores(seed=1), 4)
+    for name, call in _terms(top).items():
+        x = _scores(seed=2).requires_grad_(True)
+        (g,) = torch.autograd.grad(call(x), x, create_graph=True)
+        assert g.abs().sum() > 0, name
+        with pytest.raises(RuntimeError, match="once"):
+            torch.autograd.grad(g.square().sum() + x.square().sum(), x)
+            pytest.fail(name)
