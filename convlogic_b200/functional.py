@@ -292,6 +292,13 @@ class TopLogitsFunction(Function):
 class DistillationFunction(Function):
     """Loss of scores against a teacher's lists of top logits (``ops.distill_fwd``); the lists and the weight get no gradient."""
 
+    @classmethod
+    def apply(cls, scores, values, indices, rest, weight, temperature, reduction):  # (within forward nothing needs a gradient any more)
+        for t, what in ((values, "the lists' values"), (rest, "the rest's mass"), (weight, "the weight")):
+            if t is not None and t.requires_grad and torch.is_grad_enabled():
+                raise RuntimeError(f"convlogic_b200: {what} gets no gradient: detach it")
+        return super().apply(scores, values, indices, rest, weight, temperature, reduction)
+
     @staticmethod
     def forward(ctx, scores, values, indices, rest, weight, temperature, reduction):
         loss, stats, listed = ops.distill_fwd(scores, values, indices, rest, weight, temperature, reduction)

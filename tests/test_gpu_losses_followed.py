@@ -34,3 +34,23 @@ def test_a_second_derivative_is_refused_wherever_the_first_came_from():
         with pytest.raises(RuntimeError, match="once"):
             torch.autograd.grad(g.square().sum() + x.square().sum(), x)
             pytest.fail(name)
+
+
+def test_lists_and_weights_that_need_a_gradient_are_refused_in_a_trace():
+    import convlogic_b200 as cb
+
+    x, top = _scores(), cb.top_logits(_scores(seed=1), 4)
+
+    def call(s, values, rest, weight):
+        return cb.distillation_loss(s, (values, top.indices, rest), weight=weight)
+
+    args = (x, top.values, top.rest, torch.ones(12, device="cuda"))
+    traced = torch.jit.trace(call, args, check_trace=False)
+    for at in range(1, 4):
+        bad = list(args)
+        bad[at] = bad[at].clone().requires_grad_(True)
+        for run in (lambda: torch.jit.trace(call, tuple(bad), check_trace=False), lambda: traced(*bad)):
+            with pytest.raises(RuntimeError, match="no gradient"):
+                run()
+        with torch.no_grad():
+            assert torch.equal(traced(*bad), call(*args))
