@@ -1314,14 +1314,18 @@ struct BalanceNode : public Node {
     }
 };
 
+void refuse_sink(const Tensor &x)
+{
+    if (g_sinks.load(std::memory_order_relaxed) <= 0) return;
+    py::gil_scoped_acquire gil;
+    TORCH_CHECK(!sink_of(x), "convlogic_b200: these logits' gradient is written straight into a bucket by their layer (GradBucket.direct), "
+                             "which would overwrite the balance loss's: turn it off with direct(False)");
+}
+
 std::tuple<Tensor, Tensor> balance_loss(const Tensor &x_in, int64_t k, const std::optional<Tensor> &keep)
 {
     if (followed({x_in})) return in_python("followed_balance_loss", x_in, k, keep).cast<std::tuple<Tensor, Tensor>>();
-    if (g_sinks.load(std::memory_order_relaxed) > 0 && wants_grad({x_in})) {
-        py::gil_scoped_acquire gil;
-        TORCH_CHECK(!sink_of(x_in), "convlogic_b200: these logits' gradient is written straight into a bucket by their layer (GradBucket.direct), "
-                                    "which would overwrite the balance loss's: turn it off with direct(False)");
-    }
+    if (wants_grad({x_in})) refuse_sink(x_in);
     Balanced out;
     {
         const Tensor plain = x_in.detach();
@@ -1567,6 +1571,7 @@ PYBIND11_MODULE(_clb_torch, m)
     m.def("balance_loss", &balance_loss);
     m.def("balance_fwd", &balance_fwd_py);
     m.def("balance_bwd", &balance_bwd_py);
+    m.def("refuse_sink", &refuse_sink);
     m.def("once", [](const Tensor &g, const Tensor &x) { return once(g, x)[0]; });
     m.def("transpose2d", &transpose2d);
     m.def("adam_step", &adam_step);

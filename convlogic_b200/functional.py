@@ -315,6 +315,12 @@ class DistillationFunction(Function):
 class BalanceFunction(Function):
     """(balance loss, counts) of rows of logits over experts (``ops.balance_fwd``); the gradient goes through the probabilities."""
 
+    @classmethod
+    def apply(cls, logits, top_k, keep):
+        if torch.is_grad_enabled() and logits.requires_grad:
+            native().refuse_sink(logits)
+        return super().apply(logits, top_k, keep)
+
     @staticmethod
     def forward(ctx, logits, top_k, keep):
         loss, counts, share = ops.balance_fwd(logits, top_k, keep)

@@ -54,3 +54,37 @@ def test_lists_and_weights_that_need_a_gradient_are_refused_in_a_trace():
                 run()
         with torch.no_grad():
             assert torch.equal(traced(*bad), call(*args))
+
+
+def _direct():
+    """A layer whose gradient is written straight into a bucket."""
+    import convlogic_b200 as cb
+
+    net = torch.nn.Sequential(cb.LogicLayer(64, 400), cb.GroupSum(10, 3.0)).cuda().train()
+    bucket = cb.GradBucket(net)
+    return net, bucket, net[0].weights
+
+
+def test_a_trace_does_not_lose_a_balance_loss_beside_direct_gradients():
+    import convlogic_b200 as cb
+
+    net, bucket, w = _direct()
+
+    class Balance(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.w = w
+
+        def forward(self, scale):
+            return cb.balance_loss(self.w)[0] * scale
+
+    one = torch.ones((), device="cuda")
+    early = torch.jit.trace(Balance(), (one,), check_trace=False)
+    bucket.direct()
+    for call in (lambda: torch.jit.trace(Balance(), (one,), check_trace=False), lambda: early(one)):
+        with pytest.raises(RuntimeError, match="direct"):
+            call()
+    with torch.no_grad():
+        early(one)
+    bucket.direct(False)
+    assert torch.equal(early(one), cb.balance_loss(w)[0])
