@@ -1314,11 +1314,11 @@ struct BalanceNode : public Node {
     }
 };
 
-void refuse_sink(const Tensor &x)
+void refuse_sink(const Tensor &x) // x or what it is a view of
 {
     if (g_sinks.load(std::memory_order_relaxed) <= 0) return;
     py::gil_scoped_acquire gil;
-    TORCH_CHECK(!sink_of(x), "convlogic_b200: these logits' gradient is written straight into a bucket by their layer (GradBucket.direct), "
+    TORCH_CHECK(!sink_of(x) && !(x.is_view() && sink_of(Tensor(at::TensorBase(x._base())))), "convlogic_b200: these logits' gradient is written straight into a bucket by their layer (GradBucket.direct), "
                              "which would overwrite the balance loss's: turn it off with direct(False)");
 }
 

@@ -88,3 +88,23 @@ def test_a_trace_does_not_lose_a_balance_loss_beside_direct_gradients():
         early(one)
     bucket.direct(False)
     assert torch.equal(early(one), cb.balance_loss(w)[0])
+
+
+def test_views_of_a_parameter_are_refused_beside_direct_gradients():
+    import convlogic_b200 as cb
+
+    net, bucket, w = _direct()
+    views = (lambda: w.view(40, 10, 16), lambda: w[:100], lambda: w.view(-1, 16)[3:].unsqueeze(0), lambda: w.t(), lambda: w.detach().requires_grad_(True))
+    before = [cb.balance_loss(v())[0].detach() for v in views]
+    bucket.direct()
+    for v in views[:-1]:
+        with pytest.raises(RuntimeError, match="direct"):
+            cb.balance_loss(v())
+        with torch.no_grad():
+            cb.balance_loss(v())
+    assert torch.equal(cb.balance_loss(views[-1]())[0].detach(), before[-1])     # no longer the parameter's
+    scores = net(torch.rand(50, 64, device="cuda"))
+    cb.balance_loss(scores)[0].backward()                                        # logits that a layer has made
+    bucket.direct(False)
+    for v, b in zip(views, before):
+        assert torch.equal(cb.balance_loss(v())[0].detach(), b)
