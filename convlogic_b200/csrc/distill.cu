@@ -776,7 +776,11 @@ extern "C" int clb_distill_fwd(const void *scores, int64_t row_stride, const flo
             using T = decltype(t);
             rc = run_fwd<T>((const T *)scores, p, (T *)grad, make_args(rows, classes, row_stride, k, temperature, reduction), st);
         });
-        if (rc != cudaSuccess) return check_launch(0);
+        if (rc != cudaSuccess) { // (whatever the last error is by now)
+            set_last_cuda_error((int)rc);
+            cudaGetLastError();
+            return CLB_ERR_LAUNCH;
+        }
     }
     if (reduction == CLB_REDUCE_NONE) return rows > 0 ? check_launch() : CLB_OK;
     if (rows <= kOneSum) {
