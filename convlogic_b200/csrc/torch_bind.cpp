@@ -1149,12 +1149,15 @@ variable_list once(Tensor g, const Tensor &x)
 
 Tensor plain_float(const Tensor &t) { return t.scalar_type() == at::kFloat && t.is_contiguous() ? t : t.detach().to(at::kFloat).contiguous(); }
 
-// Which capture the current stream records into, 0 for none.
+// Which capture the current stream records into, 0 for none.  (The default stream, which cannot be captured, is not asked: the question costs, and may fail while another
+// stream is captured.)
 unsigned long long capture_id()
 {
+    const cudaStream_t stream = c10::cuda::getCurrentCUDAStream();
+    if (!stream) return 0;
     cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
     unsigned long long id = 0;
-    TORCH_CHECK(cudaStreamGetCaptureInfo(c10::cuda::getCurrentCUDAStream(), &status, &id) == cudaSuccess, "convlogic_b200: the stream cannot be asked for its capture");
+    TORCH_CHECK(cudaStreamGetCaptureInfo(stream, &status, &id) == cudaSuccess, "convlogic_b200: the stream cannot be asked for its capture");
     return status == cudaStreamCaptureStatusActive ? id : 0;
 }
 

@@ -1,4 +1,4 @@
-"""What the loss terms answer where no launch can succeed, and to what a data loader makes of their lists: on the host."""
+"""What the loss terms answer where no launch can succeed, on the host."""
 
 import os
 import subprocess
