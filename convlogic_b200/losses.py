@@ -49,8 +49,9 @@ def distillation_loss(scores, top, temperature=1.0, weight=None, reduction="mean
 
     scores [..., classes] float32, float16 or bfloat16; the loss is float32, the gradient has the scores' type."""
     if isinstance(top, TopLogits):
-        if top.temperature is not None and top.temperature != temperature:
-            raise ValueError(f"the lists were made at temperature {top.temperature}, the loss is taken at {temperature}")
+        made = top.temperature  # (one for each sample where a data loader has put samples' lists together)
+        if made is not None and ((made != temperature).any() if isinstance(made, torch.Tensor) else made != temperature):
+            raise ValueError(f"the lists were made at temperature {made}, the loss is taken at {temperature}")
         values, indices, rest = top[:3]
     else:
         if len(top) not in (2, 3):
