@@ -381,13 +381,14 @@ template <typename F> void with_team(int64_t experts, F &&f)
     else if (experts <= 512) f(integral_constant<int, 32>(), integral_constant<int, 16>());
     else f(integral_constant<int, 32>(), integral_constant<int, 32>());
 }
-// Blocks of the forward pass: those that are resident, and sums of at most 512 KB for the one block that finishes.  (Of 148 SMs: what the scratch is for.)
+// Blocks of the forward pass: those that are resident.  (Of 148 SMs: what the scratch is for.)  With the sums held to 512 KB, when one block finished them, most SMs were
+// idle from 384 experts on, us, k = 8, forward and finish: 65536 rows of 384 132 + 11, now 75 + 13; of 1024 919 + 11, now 228 + 21; 4096 of 1024 58 + 11, now 22 + 20.
 int balance_blocks(int64_t rows, int64_t experts)
 {
     int64_t n = 0;
     with_team(experts, [&](auto G, auto NC) {
         const int64_t teams = kThreads<decltype(NC)::value> / decltype(G)::value;
-        n = std::min<int64_t>((rows + teams - 1) / teams, std::min<int64_t>(148 * kResident<decltype(G)::value, decltype(NC)::value>, std::max<int64_t>(64, 65536 / experts)));
+        n = std::min<int64_t>((rows + teams - 1) / teams, 148 * kResident<decltype(G)::value, decltype(NC)::value>);
     });
     return (int)n;
 }

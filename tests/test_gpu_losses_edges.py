@@ -6,7 +6,7 @@ import pytest
 import torch
 
 from oracle import loss_oracle
-from tests.test_gpu_losses import DTYPES, EPS, IDS, check_distill, check_grad, check_loss, check_top, lists_for, made
+from tests.test_gpu_losses import DTYPES, EPS, IDS, check_balance, check_distill, check_grad, check_loss, check_top, lists_for, made
 
 pytestmark = pytest.mark.gpu
 
@@ -159,3 +159,17 @@ def test_top_logits_just_past_a_size(v, k, more, dtype):
     check_top(made(40, v + 9, dtype, "wide")[:, 3:3 + v], k, 2.0)
     short, long = (torch.randn(8192 if v < 8192 else 2048, w, device="cuda").to(dtype) for w in (v, more))
     assert _time(lambda: cb.top_logits(short, k)) < 2.0 * _time(lambda: cb.top_logits(long, k))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("e", [385, 1024])
+def test_balance_of_many_experts_and_rows(e, dtype):
+    """All blocks that are resident take part, whatever the number of experts: twice the experts take no more than three times as long."""
+    import convlogic_b200 as cb
+
+    x = made(3000, e, dtype, "normal")
+    check_balance(x, 3)
+    many = torch.randn(65536, e, device="cuda").to(dtype)
+    half = many[:, :e // 2].contiguous()
+    assert _time(lambda: cb.balance_loss(many)) < 3.0 * _time(lambda: cb.balance_loss(half))
+    assert int(cb.balance_loss(many, 8)[1].sum()) == 8 * 65536
