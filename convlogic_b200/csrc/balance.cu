@@ -371,8 +371,7 @@ __global__ void __launch_bounds__(kThreads<NC>, kResident<G, NC>) balance_bwd_ke
 template <typename F> void with_team(int64_t experts, F &&f)
 {
     using std::integral_constant;
-    if (experts <= 4) f(integral_constant<int, 1>(), integral_constant<int, 8>());
-    else if (experts <= 8) f(integral_constant<int, 1>(), integral_constant<int, 8>());
+    if (experts <= 8) f(integral_constant<int, 1>(), integral_constant<int, 8>());
     else if (experts <= 16) f(integral_constant<int, 1>(), integral_constant<int, 16>());
     else if (experts <= 32) f(integral_constant<int, 2>(), integral_constant<int, 16>());
     else if (experts <= 64) f(integral_constant<int, 4>(), integral_constant<int, 16>());

@@ -727,7 +727,8 @@ template <typename T> cudaError_t run_fwd(const T *x, const FwdPointers &p, T *g
     if (pieces <= 32 * NV) return launch_fwd<T, 32, NV, false>(x, p, grad, a, 0, pieces, st);
     // A row of up to 16384 values in a block's registers where it fills most of them, else through the block twice.  134 million values with their gradient and
     // lists of 64, registers / twice: 8192 of 8192 values fp32 260 / 285 us, bf16 206 / 251; 16384 of 16384 249 / 219, bf16 203 / 217; 4096 of 8192 418 / 382, bf16
-    // 371 / 246.  (A few rows are shared by clusters instead.)
+    // 371 / 246.  A few rows are shared by clusters instead, which is even at 64 rows and twice the time from 150 on.  Clusters / twice, bf16: 64 rows of 50257 14 / 18,
+    // of 131072 21 / 24, of 390000 78 / 49; 100 rows 21 / 18, 36 / 26, 109 / 53; 148 rows 28 / 19, 44 / 26, 154 / 66; 296 rows 46 / 24, 84 / 42, 302 / 126.
     const long long room = (pieces <= 128 * NV ? 128 : 256) * NV;
     const bool many = a.rows >= 64 && a.classes <= 400000; // (two tables of 49 KB)
     if (pieces <= block && (!many || 10 * pieces >= 7 * room))
