@@ -31,7 +31,7 @@ def top_logits(logits, k, temperature=1.0):
     """The ``k`` largest of every row of ``logits`` [..., classes] as ``TopLogits``: values float32 [..., k] in descending order, indices int64
     [..., k], rest float32 [...].  Equal values are listed by index, NaN before every number; ``rest`` is -inf where nothing is left.
 
-    float32, float16 or bfloat16, any distance between rows; 1 <= k <= min(classes, 128).  No gradient."""
+    float32, float16 or bfloat16 (not float64), any distance between rows; 1 <= k <= min(classes, 128).  No gradient."""
     return TopLogits(*native().top_logits(logits, k, float(temperature)), float(temperature))
 
 
@@ -47,7 +47,11 @@ def distillation_loss(scores, top, temperature=1.0, weight=None, reduction="mean
     teacher mass (values and rest all -inf) or with scores that are all -inf.  ``reduction``: "none" (one loss for each row), "sum", or
     "mean", which divides by the number of rows, weighted or not (over the rows kept: ``weight=keep / keep.sum()`` with "sum").  No rows: 0.
 
-    scores [..., classes] float32, float16 or bfloat16; the loss is float32, the gradient has the scores' type."""
+    scores [..., classes] float32, float16 or bfloat16 (not float64: ``scores.float()``); the loss is float32, the gradient has the scores' type.
+
+    The forward call writes the gradient for an upstream gradient of one, beside the loss (not for float16, nor with "none"); any other is computed by
+    the backward call, which reads the scores again: ``0.5 * loss`` takes about 1.8 times as long as ``loss`` on long rows.  A coefficient within
+    ``weight`` (``torch.full([rows], 0.5)``) costs nothing.  Under ``no_grad`` only the loss is computed."""
     if isinstance(top, TopLogits):
         made = top.temperature  # (one for each sample where a data loader has put samples' lists together)
         if made is not None and ((made != temperature).any() if isinstance(made, torch.Tensor) else made != temperature):
@@ -61,13 +65,14 @@ def distillation_loss(scores, top, temperature=1.0, weight=None, reduction="mean
 
 
 def balance_loss(logits, top_k=1, keep=None):
-    """(loss, counts) of rows of ``logits`` [..., experts] that choose their ``top_k`` largest (equal ones by index; never a logit of -inf):
+    """(loss, counts) of rows of ``logits`` [..., experts] that choose their ``top_k`` largest (equal ones by index; never a logit of -inf; NaN counts as +inf and
+    makes the loss and its row's gradient NaN):
 
     counts int64 [experts]: the rows that choose an expert; loss = experts / (rows * top_k) * sum_e counts[e] * mean probability of e, which is 1
     where choices and probabilities are even.  The gradient goes through the probabilities, the counts have none.
 
     ``keep`` bool [...]: the rows that count (a padded batch); rows without a logit above -inf never do.  No rows: 0.  float32, float16 or
-    bfloat16; at most 1024 experts, top_k at most 32.
+    bfloat16 (not float64: ``logits.float()``); at most 1024 experts, top_k at most 32.
 
     For a layer's gates pass its ``weights`` ([..., 16]): the counts are then the operations of the discretised layer.  Not with
     ``GradBucket.direct()``, where a parameter's gradient is written by one backward call alone: that raises."""

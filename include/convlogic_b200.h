@@ -438,7 +438,8 @@ int clb_top_logits(const void *x, int64_t row_stride, float *values, int64_t *in
  *   loss = temperature^2 weight [ sum_k p_k (log p_k - log q_{i_k}) + r (log r - log q_r) ]     (nothing for a probability of zero).
  * rest [rows] may be NULL (the listed classes are then all that the teacher knows: r = 0), weight [rows] may be NULL (ones).  An entry of
  * a list whose index is outside [0, classes) does not exist; an index that is listed twice has both entries' probability.  A row of weight zero, of no
- * teacher mass or of scores that are all -inf adds nothing and gets a gradient of zero, whatever else it holds.
+ * teacher mass or of scores that are all -inf adds nothing and gets a gradient of zero, whatever else it holds.  Where a listed class has a probability and its
+ * score is -inf, or so low that (scores - largest) / temperature or the row's loss leaves the floats, the loss is +inf; the gradient is not.
  * reduction: CLB_REDUCE_NONE (loss [rows]), CLB_REDUCE_MEAN (loss [1], the sum divided by rows) or CLB_REDUCE_SUM (loss [1]); zero rows add up to zero.
  * The forward leaves stats [rows][2] and listed [rows][k] for the backward, and writes d loss / d scores for an upstream gradient of one into grad, from
  * the scores that it holds for the loss, unless grad is NULL.
@@ -456,7 +457,7 @@ int clb_distill_bwd(const void *scores, int64_t row_stride, const int64_t *indic
                     int upstream_per_row, int unit_done, void *grad, int64_t rows, int64_t classes, int k, double temperature, int dtype, void *stream);
 
 /* Balance loss over experts (the 16 operations of a layer's gates, the experts of a router): with p = softmax(x) and the k largest logits of a
- * row its choices (equal ones by index, never a logit of -inf), counts[e] = rows that choose e, M = kept rows,
+ * row its choices (equal ones by index, never a logit of -inf; NaN counts as +inf, and makes the loss and its row's gradient NaN), counts[e] = rows that choose e, M = kept rows,
  *   loss = experts / (M k) * sum_e counts[e] * mean of p_e over the kept rows.
  * Kept are the rows with keep[r] != 0 (keep may be NULL: all) that have a logit above -inf; M = 0: loss 0.  counts int64 [experts], loss [1]; share
  * [experts] is what the backward needs: grad = upstream * p_j (share_j - sum_e p_e share_e), the gradient through p, zero for rows that are not kept.

@@ -173,3 +173,31 @@ def test_balance_of_many_experts_and_rows(e, dtype):
     half = many[:, :e // 2].contiguous()
     assert _time(lambda: cb.balance_loss(many)) < 3.0 * _time(lambda: cb.balance_loss(half))
     assert int(cb.balance_loss(many, 8)[1].sum()) == 8 * 65536
+
+
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("e,k", [(5, 2), (16, 1), (16, 6), (60, 3), (128, 8), (700, 5)])
+def test_balance_of_rows_with_nan(e, k, dtype):
+    """NaN counts as +inf, by index; the loss and such a row's gradient are NaN, the other rows' are as they are.  A row with both has them chosen by index, too."""
+    import convlogic_b200 as cb
+
+    inf, nan = float("inf"), float("nan")
+    x = made(40, e, dtype, "normal")
+    x[3, e // 2] = nan
+    x[4, 1::2] = nan
+    x[5, 0], x[5, e - 1] = inf, nan
+    x[6, 0], x[6, e - 1] = nan, inf
+    x[7], x[7, e // 3] = -inf, nan
+    x[8, e // 2] = inf
+    leaf = x.clone().requires_grad_(True)
+    loss, counts = cb.balance_loss(leaf, k)
+    (g,) = torch.autograd.grad(loss, leaf)
+    want = loss_oracle.balance(x.float().nan_to_num(inf, inf, -inf), k)["counts"]
+    assert torch.equal(counts.cpu(), want) and torch.isnan(loss)
+    assert torch.isnan(g[3:9]).any(1).all()
+    p = torch.softmax(x.double(), 1)
+    h = e / (40.0 * 40 * k) * (counts.double() - counts.double().mean())
+    fine = torch.cat([torch.arange(3), torch.arange(9, 40)]).cuda()
+    exact = (p * (h - (p * h).sum(1, keepdim=True)))[fine].cpu()
+    scale = (p * (h.abs() + (p * h.abs()).sum(1, keepdim=True)))[fine].cpu()
+    check_grad(g[fine], exact, scale, dtype)
