@@ -41,6 +41,7 @@ struct TeacherNumbers {
     float m, ref, tl; // its mass is tl * exp(m / T + ref)
     float d;          // log of the rest's mass, less m / T
     float rest;       // probability of the rest
+    float listed;     // and of all that is listed
     float factor;     // of the row's loss / T and gradient; 0: the row adds nothing
     __device__ __forceinline__ float log_p(float t, float tt, float log_tl) const { return ((t - m) / tt - ref) - log_tl; }
 };
@@ -56,8 +57,9 @@ __device__ __forceinline__ TeacherNumbers teacher_numbers(ExpSum teach, float rs
         q.d = rs == -INFINITY ? rs : rs - rs;
     q.ref = finite_or_zero(fmaxf(none ? -INFINITY : 0.f, q.d));
     const float re = ex2((q.d - q.ref) * 1.44269504f);
-    q.tl = (none ? teach.l : teach.l * ex2(-q.ref * 1.44269504f)) + re;
-    q.rest = re / q.tl;
+    const float all = none ? teach.l : teach.l * ex2(-q.ref * 1.44269504f);
+    q.tl = all + re;
+    q.rest = re / q.tl, q.listed = all / q.tl;
     q.factor = q.tl != 0.f ? w * a.scale : 0.f;
     return q;
 }
@@ -90,9 +92,12 @@ __device__ __forceinline__ RowNumbers row_numbers(ExpSum rest, ExpSum list, cons
     RowNumbers n; // (a sum of 0 has no terms: the largest adds 1)
     n.m = finite_or_zero(rest.m), n.um = finite_or_zero(fmaxf(rest.m, list.m)), n.l = rest.l;
     const float of_rest = rest.l == 0.f ? 0.f : rest.l * exp_of(n.m, n.um, a.c);
-    n.ul = of_rest + (list.l == 0.f ? 0.f : list.l * exp_of(finite_or_zero(list.m), n.um, a.c));
+    const float of_list = list.l == 0.f ? 0.f : list.l * exp_of(finite_or_zero(list.m), n.um, a.c);
+    n.ul = of_rest + of_list;
     n.qr = __fdividef(of_rest, n.ul);
-    n.coef = q.factor == 0.f || rest.l == 0.f ? 0.f : q.factor * __fdividef(n.qr - q.rest, rest.l);
+    // q_r - r, or the same by what is listed where that is less: two numbers near one leave 2^-24 of one
+    const float more = n.qr + q.rest > 1.f ? q.listed - __fdividef(of_list, n.ul) : n.qr - q.rest;
+    n.coef = q.factor == 0.f || rest.l == 0.f ? 0.f : q.factor * __fdividef(more, rest.l);
     return n;
 }
 
@@ -359,6 +364,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH)
     const int words = a.chunks * WORDS * MT;
     __shared__ ExpSum part[32];
     __shared__ float4 from_list; // maximum and sum of the distinct listed scores, the teacher's probability of the rest, the gradient's factor
+    __shared__ float p_listed;   // the teacher's probability of all listed classes
     __shared__ int list[CLB_TOP_MAX];
     const int t = threadIdx.x, lane = t & 31, warp = t >> 5;
     const float tt = a.temperature;
@@ -445,7 +451,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH)
             }
             sk.l = lanes_sum<32>(sk.l), tk.l = lanes_sum<32>(tk.l);
             const TeacherNumbers q = teacher_numbers(tk, rs, w, a);
-            if (lane == 0) from_list = make_float4(sk.m, sk.l, q.rest, q.factor);
+            if (lane == 0) from_list = make_float4(sk.m, sk.l, q.rest, q.factor), p_listed = q.listed;
             __syncthreads(); // ------------ all sums are there
             const RowNumbers n = row_numbers(lanes_merge<32>(part[lane], a.c), sk, q, a);
             const bool there = q.factor != 0.f && n.ul != 0.f;
@@ -542,7 +548,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH)
         if (grad) {
             const float4 l = from_list;
             TeacherNumbers q;
-            q.rest = l.z, q.factor = l.w;
+            q.rest = l.z, q.factor = l.w, q.listed = p_listed;
             const RowNumbers n = row_numbers(lanes_merge<32>(part[lane], a.c), ExpSum{l.x, l.y}, q, a);
             T *out = grad + r * a.classes;
             const bool aligned = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(row.row)) & 15) == 0;

@@ -131,6 +131,31 @@ def test_losses_near_zero(n, v, k):
         assert ((loss - want["loss"]).abs() <= bound).all(), (noise, loss, want["loss"], bound)
 
 
+@pytest.mark.parametrize("n,v,k", [(8, 12, 1), (8, 100, 2), (8, 1000, 1), (8, 5000, 16), (3, 70001, 1), (3, 140003, 32), (66, 2100, 1), (66, 20000, 1), (66, 40001, 100)])
+def test_gradients_of_lists_that_hold_little(n, v, k):
+    """An unlisted class's gradient is T q_j (q_r - r) / q_r.  Where r and q_r are near one their difference is that of the listed probabilities, P - Q, each EPS off, and the other
+    factors are EPS off: T q_j / q_r (EPS (P + Q) + 3 EPS |P - Q|)."""
+    import convlogic_b200 as cb
+
+    t = 4.0
+    g = torch.Generator().manual_seed(v * k)
+    x = torch.randn(n, v, generator=g).double()
+    teacher = x + torch.randn(n, v, generator=g)
+    values, indices, rest = loss_oracle.top_logits(teacher, k, t)
+    top = (values.float().cuda(), indices.cuda(), rest.float().cuda())
+    p = torch.softmax(torch.cat([top[0].cpu().double() / t, top[2].cpu().double()[:, None]], 1), 1)[:, :-1].sum(1, keepdim=True)
+    for reduction in ("sum", "none"):
+        leaf = x.float().cuda().requires_grad_(True)
+        loss = cb.distillation_loss(leaf, top, t, reduction=reduction)
+        (grad,) = torch.autograd.grad(loss, leaf, torch.ones_like(loss))
+        s = torch.softmax(leaf.detach().cpu().double() / t, 1)
+        q = s.gather(1, indices).sum(1, keepdim=True)
+        want = t * s / (1 - q) * (p - q)
+        bound = t * s / (1 - q) * EPS * ((p + q) + 3 * (p - q).abs())
+        off = ((grad.cpu().double() - want).abs() - bound).scatter(1, indices, -1.0)
+        assert (off <= 0).all(), (reduction, off.max())
+
+
 # ------------------------------------------------------------------------------------------------ sizes just past a kernel's
 def _time(call, n=5):
     """The shortest of five times of a call, each the mean of n."""
