@@ -59,7 +59,7 @@ __device__ __forceinline__ TeacherNumbers teacher_numbers(ExpSum teach, float rs
     const float re = ex2((q.d - q.ref) * 1.44269504f);
     const float all = none ? teach.l : teach.l * ex2(-q.ref * 1.44269504f);
     q.tl = all + re;
-    q.rest = re / q.tl, q.listed = all / q.tl;
+    q.rest = __fdividef(re, q.tl), q.listed = __fdividef(all, q.tl);
     q.factor = q.tl != 0.f ? w * a.scale : 0.f;
     return q;
 }
@@ -69,10 +69,10 @@ __device__ __forceinline__ TeacherNumbers teacher_numbers(ExpSum teach, float rs
 __device__ __forceinline__ float share_of(float p, float delta, float q)
 {
     if (p == 0.f) return q;
-    if (!(fabsf(delta) < 0.5f)) return p * (delta - 1.f) + q;
-    const float d = delta; // exp(-d) - 1 + d, Taylor's
-    float f = fmaf(d, -1.f / 362880, 1.f / 40320);
-    f = fmaf(d, f, -1.f / 5040), f = fmaf(d, f, 1.f / 720), f = fmaf(d, f, -1.f / 120), f = fmaf(d, f, 1.f / 24), f = fmaf(d, f, -1.f / 6), f = fmaf(d, f, 0.5f);
+    if (!(fabsf(delta) < 0.25f)) return p * (delta - 1.f) + q;
+    const float d = delta; // exp(-d) - 1 + d, Taylor's to d^7: the next term is 2e-8 of the first
+    float f = fmaf(d, -1.f / 5040, 1.f / 720);
+    f = fmaf(d, f, -1.f / 120), f = fmaf(d, f, 1.f / 24), f = fmaf(d, f, -1.f / 6), f = fmaf(d, f, 0.5f);
     return p * (d * d) * f;
 }
 // What a row's sums come to: unlisted scores `rest`, distinct listed ones `list`.
@@ -80,11 +80,10 @@ struct RowNumbers {
     float m, l, coef;  // of the unlisted scores: reference and sum; gradient = coef * exp((s - m) / T).  The list's = factor * (q - p)
     float um, ul;      // of all scores; ul = 0: there are none
     float qr;          // probability of the unlisted ones
-    __device__ __forceinline__ float loss(float listed, const TeacherNumbers &q, float tt) const // listed: the list's terms
+    __device__ __forceinline__ float rest_share(const TeacherNumbers &q, float tt, float log_tl, float log_ul) const // of the row's loss / (factor * T)
     {
-        const float log_qr = l == 0.f ? -INFINITY : ((m - um) / tt + logf(l)) - logf(ul);
-        listed += share_of(q.rest, ((q.d - q.ref) - logf(q.tl)) - log_qr, qr);
-        return listed * q.factor * tt;
+        const float log_qr = l == 0.f ? -INFINITY : ((m - um) / tt + logf(l)) - log_ul;
+        return share_of(q.rest, ((q.d - q.ref) - log_tl) - log_qr, qr);
     }
 };
 __device__ __forceinline__ RowNumbers row_numbers(ExpSum rest, ExpSum list, const TeacherNumbers &q, const DistillArgs &a)
@@ -340,7 +339,7 @@ __global__ void __launch_bounds__(TH <= 32 ? 256 : TH, TH > 32 ? 512 / TH : NV *
                 loss = 0.f;
                 for (int i = 0; i < list_warps; ++i) loss += loss_part[i];
             }
-            row_loss[r] = there ? num.loss(loss, teach, tt) : 0.f;
+            row_loss[r] = there ? (loss + num.rest_share(teach, tt, log_tl, log_ul)) * teach.factor * tt : 0.f;
             stats[2 * r] = m, stats[2 * r + 1] = coef;
         }
         team_sync(); // the tables are used again
@@ -456,7 +455,8 @@ __global__ void __launch_bounds__(TH, 1024 / TH)
             const RowNumbers n = row_numbers(lanes_merge<32>(part[lane], a.c), sk, q, a);
             const bool there = q.factor != 0.f && n.ul != 0.f;
             const float log_tl = logf(q.tl), log_ul = logf(n.ul);
-            float loss = 0.f;
+            float loss = n.rest_share(q, tt, log_tl, log_ul); // (beside the list's terms, not behind their sum)
+            loss = lane == 0 ? loss : 0.f;
 #pragma unroll
             for (int i = 0; i < EACH; ++i) {
                 g[i] = 0.f;
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(TH, 1024 / TH)
             }
             loss = lanes_sum<32>(loss);
             if (lane == 0) {
-                row_loss[r] = there ? n.loss(loss, q, tt) : 0.f;
+                row_loss[r] = there ? loss * q.factor * tt : 0.f;
                 stats[2 * r] = n.m, stats[2 * r + 1] = n.coef;
             }
             next_dup = mark(r + gridDim.x, tables + (odd ^ 1) * words);
