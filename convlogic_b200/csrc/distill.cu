@@ -11,8 +11,8 @@
 //
 // A team of threads holds the row in registers (clb_rows.cuh): one read of the scores, a maximum, a sum, and the gradient from the same registers.  Listed
 // classes are struck out there: a bit per value in shared memory, set by the threads that hold the list.  Many rows that are longer than a block's registers go
-// through a block twice (distill_stream_kernel).  With the gradient: 8192 rows of 1000 fp32 21 us (3.1 TB/s; bound by issue, the list costs a warp as much as its
-// row), 2048 of 131072 bf16 245 us (4.4 TB/s; reading, reading again from the L2 and writing alone take 203).
+// through a block twice (distill_stream_kernel).  With the gradient: 8192 rows of 1000 fp32 22 us (3.0 TB/s; bound by issue, the list costs a warp as much as its
+// row), 2048 of 131072 bf16 243 us (4.4 TB/s; reading, reading again from the L2 and writing alone take 203).
 #include <cooperative_groups.h>
 
 #include "clb_rows.cuh"
