@@ -51,7 +51,7 @@ __device__ __forceinline__ TeacherNumbers teacher_numbers(ExpSum teach, float rs
     const bool none = teach.m == -INFINITY;
     q.m = finite_or_zero(teach.m);
     if (fabsf(rs) < INFINITY) { // m / T by a reciprocal in two parts: rounded, it would be off by 2^-24 of itself
-        const float of_m = q.m * a.inv;
+        const float of_m = __fmul_rn(q.m, a.inv); // (not to become part of the difference, which takes what it is rounded by on its own)
         q.d = fabsf(of_m) < INFINITY ? fminf((rs - of_m) - fmaf(q.m, a.inv, -of_m) - q.m * a.inv_low, 3.402823466e38f) : copysignf(3.402823466e38f, -of_m);
     } else
         q.d = rs == -INFINITY ? rs : rs - rs;
