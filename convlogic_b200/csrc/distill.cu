@@ -277,12 +277,12 @@ __global__ void __launch_bounds__(TH <= 32 ? 256 : TH, TH > 32 ? 512 / TH : NV *
             const bool aligned = ((reinterpret_cast<uintptr_t>(out) ^ reinterpret_cast<uintptr_t>(row.row)) & 15) == 0;
             for (int ch = 0; ch < chunks; ++ch) {
                 float scale = coef;
-                if (chunks == 1) scale = coef * exp_of(own_max, m, a.c);
+                if (chunks == 1) scale = coef == 0.f ? 0.f : coef * exp_of(own_max, m, a.c);
                 else {
                     fetch(ch);
                     exponentials(m);
                 }
-                if (coef == 0.f) // (a row that adds nothing may hold NaN)
+                if (coef == 0.f) // (a row that adds nothing may hold NaN and infinities)
 #pragma unroll
                     for (int i = 0; i < NV * EV; ++i) v[i] = 0.f;
                 const int base = (ch * ranks + rank) * TH * NV;

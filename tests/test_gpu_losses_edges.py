@@ -67,6 +67,34 @@ def test_distillation_of_classes_masked_with_a_number(n, v, mask, dtype):
         check_distill(x, top, 1.5, None, "sum", None)
 
 
+@pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
+@pytest.mark.parametrize("n,v", [(6, 3), (6, 12), (6, 100), (6, 300), (6, 1000), (6, 4000), (6, 12000), (6, 70001), (6, 300001), (70, 2100), (70, 12000), (66, 70001)])
+def test_infinities_in_rows_that_count_for_nothing(n, v, dtype):
+    """Weight zero, a list without mass: the gradient is zero whatever stands there, whether the forward writes it or the backward."""
+    import convlogic_b200 as cb
+
+    inf, nan = float("inf"), float("nan")
+    x = made(n, v, dtype, "normal")
+    values, indices, rest = lists_for(x, 2, 1.0)
+    weight = torch.ones(n, device="cuda")
+    for i, bad in enumerate((inf, nan, -inf)):
+        for j, row in enumerate((i, n - 1 - i)):
+            x[row, 0] = x[row, v // 2] = bad
+            x[row, :: 3 + j] = bad
+    weight[0] = weight[1] = weight[2] = 0.0
+    values[n - 3:], rest[n - 3:] = -inf, -inf
+    indices[n - 1] = -1
+    x[0, indices[0, 0]] = inf
+    nothing = torch.tensor([0, 1, 2, n - 3, n - 2, n - 1]).cuda()
+    for reduction in ("sum", "mean", "none"):
+        for up in (1.0, 0.5):
+            leaf = x.clone().requires_grad_(True)
+            loss = cb.distillation_loss(leaf, (values, indices, rest), weight=weight, reduction=reduction)
+            (g,) = torch.autograd.grad(loss, leaf, torch.full_like(loss, up))
+            assert torch.isfinite(loss).all() and not g[nothing].any() and not torch.isnan(g).any()
+            assert n == 6 or g[3:n - 3].any(1).all()
+
+
 # ------------------------------------------------------------------------------------------------ lists far from zero
 @pytest.mark.parametrize("dtype", DTYPES, ids=IDS)
 @pytest.mark.parametrize("shift", [0.0, 3e3, -1e4, 1e6])
